@@ -30,29 +30,29 @@ def _ops():
 def listed():
     return [
         # one context token per frame of a clip: the smallest norm, nothing but latency
-        dict(name="norm, context tokens", op="norm", rows=16, width=1024, dtype="bf16", wdtype="fp32", residual=False),
+        dict(name="norm context tokens", op="norm", rows=16, width=1024, dtype="bf16", wdtype="fp32", residual=False),
         # the residual stream of the 1024^2 stage's widest level (16 frames of 128 x 128 tokens): sum, norm and statistics in one pass
-        dict(name="residual norm, 128x128", op="norm", rows=262144, width=320, dtype="bf16", wdtype="fp32", residual=True),
+        dict(name="residual norm 128x128", op="norm", rows=262144, width=320, dtype="bf16", wdtype="fp32", residual=True),
         # the backward pass one level down, the gradient of the residual stream joining it
-        dict(name="norm gradients, 64x64", op="norm_grad", rows=65536, width=640, dtype="bf16", wdtype="fp32", residual=True),
+        dict(name="norm gradients 64x64", op="norm_grad", rows=65536, width=640, dtype="bf16", wdtype="fp32", residual=True),
         # a width that no vector divides, half precision throughout
-        dict(name="norm gradients, odd", op="norm_grad", rows=7013, width=1285, dtype="fp16", wdtype="fp16", residual=False),
+        dict(name="norm gradients odd", op="norm_grad", rows=7013, width=1285, dtype="fp16", wdtype="fp16", residual=False),
         # the time embedding's second layer over a clip's frames: few rows, the weights are all there is to read
-        dict(name="linear, time embedding", op="linear", rows=16, inner=1280, outer=1280, dtype="bf16", act="silu", residual=False, save=False),
+        dict(name="linear time embedding", op="linear", rows=16, inner=1280, outer=1280, dtype="bf16", act="silu", residual=False, save=False),
         # one token, from the wide side of a feed-forward back into the residual stream
-        dict(name="linear, one token", op="linear", rows=1, inner=5120, outer=1280, dtype="bf16", act="none", residual=True, save=False),
+        dict(name="linear one token", op="linear", rows=1, inner=5120, outer=1280, dtype="bf16", act="none", residual=True, save=False),
         # the image tower's feed-forward over 16 frames of 257 tokens, its activation's argument kept for the backward pass
-        dict(name="linear, image tower", op="linear", rows=4112, inner=1280, outer=5120, dtype="bf16", act="gelu", residual=False, save=True),
+        dict(name="linear image tower", op="linear", rows=4112, inner=1280, outer=5120, dtype="bf16", act="gelu", residual=False, save=True),
         # the output side of a feed-forward at 64 x 64 tokens, added to the residual stream
-        dict(name="linear, residual 64x64", op="linear", rows=65536, inner=2560, outer=640, dtype="bf16", act="none", residual=True, save=False),
+        dict(name="linear residual 64x64", op="linear", rows=65536, inner=2560, outer=640, dtype="bf16", act="none", residual=True, save=False),
         # the backward pass of a feed-forward's input side at 32 x 32 tokens: both products and the bias
-        dict(name="linear gradients, 32x32", op="linear_grad", rows=16384, inner=1280, outer=5120, dtype="bf16", act="gelu"),
+        dict(name="linear gradients 32x32", op="linear_grad", rows=16384, inner=1280, outer=5120, dtype="bf16", act="gelu"),
         # sizes that no tile and no vector divides
-        dict(name="linear gradients, odd", op="linear_grad", rows=3083, inner=650, outer=1290, dtype="fp16", act="silu"),
+        dict(name="linear gradients odd", op="linear_grad", rows=3083, inner=650, outer=1290, dtype="fp16", act="silu"),
         # the norms and biases of a level: many short tensors
-        dict(name="adamw, norms and biases", op="adamw", tensors=60, size=960, odd=False, dtype="fp32", gdtype="fp32", copy=False),
+        dict(name="adamw norms and biases", op="adamw", tensors=60, size=960, odd=False, dtype="fp32", gdtype="fp32", copy=False),
         # a level's weights: 32-bit parameters, gradients and the working copy in 16 bits
-        dict(name="adamw, weights", op="adamw", tensors=20, size=6553600, odd=False, dtype="fp32", gdtype="bf16", copy=True),
+        dict(name="adamw weights", op="adamw", tensors=20, size=6553600, odd=False, dtype="fp32", gdtype="bf16", copy=True),
     ]
 
 
