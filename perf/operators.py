@@ -197,9 +197,8 @@ def _plain_adamw(s):
     g = [t.float() for t in s["grads"]]
     torch._foreach_mul_(s["exp_avg"], a["beta1"])
     torch._foreach_add_(s["exp_avg"], torch._foreach_mul(g, 1 - a["beta1"]))
-    torch._foreach_mul_(g, g)
     torch._foreach_mul_(s["exp_avg_sq"], a["beta2"])
-    torch._foreach_add_(s["exp_avg_sq"], torch._foreach_mul(g, 1 - a["beta2"]))
+    torch._foreach_add_(s["exp_avg_sq"], torch._foreach_mul(torch._foreach_mul(g, g), 1 - a["beta2"]))
     den = torch._foreach_sqrt(s["exp_avg_sq"])
     torch._foreach_div_(den, math.sqrt(1 - a["beta2"] ** a["step"]))
     torch._foreach_add_(den, a["eps"])
