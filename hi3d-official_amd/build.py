@@ -17,11 +17,19 @@ STAMP = LIB + ".stamp"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
          "-Wno-unused-result", "-Wno-unused-value", "-Wno-c++20-extensions", "-Rpass-analysis=kernel-resource-usage"]
+# the training kernels: fp32 arithmetic in scalar instructions only (some packed forms are not dependable on this hardware; the
+# files above them keep the code that they were measured and tested with)
+SCALAR_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+SCALAR_FP32_SOURCES = ("norm_train.hip", "linear_train.hip", "adamw.hip")
 RESOURCES = os.path.join(ROOT, "hi3d_hip", "kernel_resources.json")
 
 
 TORCH_LIB = os.path.join(ROOT, "hi3d_hip", "libhi3d_torch.so")
-TORCH_SRC = os.path.join(CSRC, "torch_ops.cpp")
+TORCH_SRCS = [os.path.join(CSRC, f) for f in ("torch_ops.cpp", "train_ops.cpp")]
+
+
+def _flags(src):
+    return FLAGS + (SCALAR_FP32 if os.path.basename(src) in SCALAR_FP32_SOURCES else [])
 
 
 def _sources():
@@ -29,12 +37,12 @@ def _sources():
 
 
 def build_torch_ops(force=False, verbose=True):
-    """libhi3d_torch.so: the TORCH_LIBRARY(hi3d, ...) shim over the C ABI (csrc/torch_ops.cpp; host-only C++, g++).
+    """libhi3d_torch.so: the TORCH_LIBRARY(hi3d, ...) shim over the C ABI (csrc/torch_ops.cpp, train_ops.cpp; host-only C++, g++).
     Linked against libhi3d_hip.so beside it ($ORIGIN rpath) and the torch libraries of THIS interpreter."""
     import torch
     tp = os.path.dirname(torch.__file__)
     h = hashlib.sha256()
-    for f in (TORCH_SRC, os.path.join(ROOT, "..", "include", "hi3d_hip.h")):
+    for f in (*TORCH_SRCS, os.path.join(ROOT, "..", "include", "hi3d_hip.h")):
         with open(f, "rb") as fh:
             h.update(fh.read())
     h.update(torch.__version__.encode())
@@ -43,11 +51,11 @@ def build_torch_ops(force=False, verbose=True):
         return TORCH_LIB
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           f"-I{tp}/include", f"-I{tp}/include/torch/csrc/api/include", "-I/opt/rocm/include", TORCH_SRC, "-o", TORCH_LIB,
+           f"-I{tp}/include", f"-I{tp}/include/torch/csrc/api/include", "-I/opt/rocm/include", *TORCH_SRCS, "-o", TORCH_LIB,
            f"-L{tp}/lib", "-lc10", "-ltorch_cpu", "-ltorch", "-lc10_hip", "-ltorch_hip", f"-L{os.path.dirname(LIB)}", "-lhi3d_hip", "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
     if r.returncode != 0:
-        raise RuntimeError("torch_ops.cpp failed to build:\n" + r.stdout.decode()[-4000:])
+        raise RuntimeError("the torch shim failed to build:\n" + r.stdout.decode()[-4000:])
     with open(stamp, "w") as fh:
         fh.write(dig)
     if verbose:
@@ -61,7 +69,7 @@ def _digest():
             os.path.join(ROOT, "..", "include", "hi3d_hip.h")]:
         with open(f, "rb") as fh:
             h.update(f.encode() + b"\0" + fh.read())
-    h.update(" ".join(FLAGS).encode())
+    h.update(" ".join(FLAGS + SCALAR_FP32 + list(SCALAR_FP32_SOURCES)).encode())
     return h.hexdigest()
 
 
@@ -110,7 +118,7 @@ def build(force=False, verbose=True):
     procs = []
     for src in _sources():
         obj = os.path.join(tmpdir, os.path.basename(src)[:-4] + ".o")
-        cmd = [HIPCC] + [f for f in FLAGS if f != "-shared"] + ["-c", src, "-o", obj]
+        cmd = [HIPCC] + [f for f in _flags(src) if f != "-shared"] + ["-c", src, "-o", obj]
         procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
         objs.append(obj)
     resources = {}
@@ -118,7 +126,7 @@ def build(force=False, verbose=True):
         out = p.communicate()[0].decode()
         if p.returncode != 0:
             raise RuntimeError(f"hipcc failed on {src}:\n{out}")
-        rest = _collect_resources(out, resources)
+        rest = "\n".join(l for l in _collect_resources(out, resources).splitlines() if "-packed-fp32-ops' is not a recognized feature" not in l)
         if verbose and rest.strip():
             print(rest, file=sys.stderr)
     with open(RESOURCES, "w") as fh:

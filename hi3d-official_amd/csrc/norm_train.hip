@@ -1,0 +1,346 @@
+// LayerNorm for training: forward with its statistics (and the residual sum in front of it), backward with the gradients of
+// weight and bias.  Beside hi3d_layernorm, which is the sampler's form of it.
+//
+//   z = x (+ residual, rounded to x's type)        mu = mean(z)   s = 1 / sqrt(mean((z - mu)^2) + eps)     h = (z - mu) s
+//   y = h w + b
+//   dz = s (w dy - mean(w dy) - h mean(w dy h)) (+ the gradient that z's other reader sends)
+//   dw = sum over rows of dy h                     db = sum over rows of dy
+//
+// Both directions are bound by HBM: every element of x and dy is read once and every element of y and dx is written once, the
+// row's sums are taken from registers (two passes over them: the variance is of the differences, so a row whose mean is
+// large against its spread keeps its digits), all in fp32.
+//
+// A row is held by LPR lanes of a wave (8 ... 64) as NV vectors of 16 bytes each, so that a wave carries 64 / LPR rows at a
+// time and a row sum is log2(LPR) steps for all of them at once; wider rows are held by the block (LPR = 256).
+#include "train_common.h"
+
+namespace {
+
+struct NormFwdParams {
+  const void* x; const void* r; const void* w; const void* b;
+  void* y; void* z; float* mean; float* rstd;
+  long R, ldx, ldr;
+  int C, wcode;
+  float eps;
+};
+struct NormBwdParams {
+  const void* dy; const void* z; const void* dz; const void* w; const float* mean; const float* rstd;
+  void* dx; float* part; void* dw; void* db;
+  long R, lddy, ldz, lddz;
+  int C, wcode, want;       // want: partial sums of dw, db are asked for
+};
+
+constexpr int NTHR = 256;
+
+// sum over the lanes that hold a row; the block form goes through LDS (`slot` alternates, so that one barrier per sum is enough)
+template <int LPR>
+__device__ __forceinline__ float row_sum(float v, float* lds, int& slot) {
+  if constexpr (LPR <= 64) return group_sum<LPR>(v);
+  v = group_sum<64>(v);
+  float* s = lds + (slot & 1) * 4;
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+  __syncthreads();
+  ++slot;
+  return (s[0] + s[1]) + (s[2] + s[3]);
+}
+
+template <typename T, int LPR, int NV, bool ADD>
+__global__ __launch_bounds__(NTHR) void norm_fwd_kernel(const NormFwdParams p) {
+  constexpr int V = Elem<T>::VEC, RPB = NTHR / LPR;
+  __shared__ float lds[8];
+  int slot = 0;
+  const int l = threadIdx.x % LPR, sub = threadIdx.x / LPR, C = p.C;
+  int n[NV];                                    // elements of this lane's i-th vector that exist
+  float w[NV][V], b[NV][V];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int e = (l + i * LPR) * V;
+    n[i] = C - e;
+#pragma unroll
+    for (int j = 0; j < V; ++j) { w[i][j] = 1.0f; b[i][j] = 0.0f; }
+    if (p.w) load_vec_as(p.w, p.wcode, e, n[i], w[i]);
+    if (p.b) load_vec_as(p.b, p.wcode, e, n[i], b[i]);
+  }
+  const bool ragged = C != LPR * NV * V;
+  const float inv = 1.0f / (float)C;
+  for (long r0 = (long)blockIdx.x * RPB; r0 < p.R; r0 += (long)gridDim.x * RPB) {
+    const long r = r0 + sub;
+    const bool in = r < p.R;                    // (a whole group of lanes at a time; the others run along on zeros)
+    float x[NV][V];
+    float s = 0.0f;
+    Pack<T, V> kx[NV], kr[ADD ? NV : 1];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      fetch((const T*)p.x + r * p.ldx + (l + i * LPR) * V, in ? n[i] : 0, kx[i]);
+      if constexpr (ADD) fetch((const T*)p.r + r * p.ldr + (l + i * LPR) * V, in ? n[i] : 0, kr[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) unpack(kx[i], x[i]);
+    if constexpr (ADD) {
+      float q[NV][V];
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        unpack(kr[i], q[i]);
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[i][j] = Elem<T>::get(Elem<T>::put(x[i][j] + q[i][j]));   // the values the backward pass reads
+        store_some((T*)p.z + r * C + (l + i * LPR) * V, in ? n[i] : 0, x[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) s += x[i][j];
+    const float mu = row_sum<LPR>(s, lds, slot) * inv;
+    if (ragged) {                               // slots behind the row differ from the mean by nothing
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[i][j] = j < n[i] ? x[i][j] : mu;
+    }
+    float q = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) { x[i][j] -= mu; q += x[i][j] * x[i][j]; }
+    const float rs = __builtin_amdgcn_rsqf(row_sum<LPR>(q, lds, slot) * inv + p.eps);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float y[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) y[j] = x[i][j] * rs * w[i][j] + b[i][j];
+      store_some((T*)p.y + r * C + (l + i * LPR) * V, in ? n[i] : 0, y);
+    }
+    if (in && l == 0) { p.mean[r] = mu; p.rstd[r] = rs; }
+  }
+}
+
+// the gradients of a block's rows: dx, and -- where they are asked for -- the block's sums of dy h and dy, in columns held by
+// the lane through all of its rows: nothing is added atomically, the order of the sums is that of the rows
+template <typename T, int LPR, int NV>
+__global__ __launch_bounds__(NTHR) void norm_bwd_kernel(const NormBwdParams p) {
+  constexpr int V = Elem<T>::VEC, RPB = NTHR / LPR;
+  __shared__ float lds[8];
+  __shared__ float cols[LPR <= 64 ? 4 * LPR * V : 1];
+  int slot = 0;
+  const int l = threadIdx.x % LPR, sub = threadIdx.x / LPR, C = p.C;
+  int n[NV];
+  float w[NV][V], gw[NV][V], gb[NV][V];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int e = (l + i * LPR) * V;
+    n[i] = C - e;
+#pragma unroll
+    for (int j = 0; j < V; ++j) { w[i][j] = 1.0f; gw[i][j] = gb[i][j] = 0.0f; }
+    if (p.w) load_vec_as(p.w, p.wcode, e, n[i], w[i]);
+  }
+  const float inv = 1.0f / (float)C;
+  for (long r0 = (long)blockIdx.x * RPB; r0 < p.R; r0 += (long)gridDim.x * RPB) {
+    const long r = r0 + sub;
+    const bool in = r < p.R;
+    Pack<T, V> ky[NV], kz[NV], kd[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      fetch((const T*)p.dy + r * p.lddy + (l + i * LPR) * V, in ? n[i] : 0, ky[i]);     // (zero behind the row: adds nothing below)
+      fetch((const T*)p.z + r * p.ldz + (l + i * LPR) * V, in ? n[i] : 0, kz[i]);
+      if (p.dz) fetch((const T*)p.dz + r * p.lddz + (l + i * LPR) * V, in ? n[i] : 0, kd[i]);
+    }
+    const float mu = in ? p.mean[r] : 0.0f, rs = in ? p.rstd[r] : 0.0f;
+    float dy[NV][V], h[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) { unpack(ky[i], dy[i]); unpack(kz[i], h[i]); }
+    float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        h[i][j] = j < n[i] ? (h[i][j] - mu) * rs : 0.0f;
+        gb[i][j] += dy[i][j];
+        gw[i][j] += dy[i][j] * h[i][j];
+        dy[i][j] *= w[i][j];
+        s1 += dy[i][j];
+        s2 += dy[i][j] * h[i][j];
+      }
+    s1 = row_sum<LPR>(s1, lds, slot) * inv;
+    s2 = row_sum<LPR>(s2, lds, slot) * inv;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float o[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) o[j] = (dy[i][j] - s1 - h[i][j] * s2) * rs;
+      if (p.dz) {
+        float t[V];
+        unpack(kd[i], t);
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] += t[j];
+      }
+      store_some((T*)p.dx + r * C + (l + i * LPR) * V, in ? n[i] : 0, o);
+    }
+  }
+  if (!p.want) return;
+  // the lanes that held the same columns: over the wave's row groups by shuffles, over the waves through LDS
+  float* part = p.part + (long)blockIdx.x * 2 * C;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      float t[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        t[j] = k ? gb[i][j] : gw[i][j];
+        if constexpr (LPR < 64) {
+#pragma unroll
+          for (int o = LPR; o < 64; o <<= 1) t[j] += __shfl_xor(t[j], o, 64);
+        }
+      }
+      if constexpr (LPR <= 64) {
+        const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+        __syncthreads();
+        if (lane < LPR) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) cols[wv * LPR * V + l * V + j] = t[j];
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < LPR * V; c += NTHR) {
+          const int e = i * LPR * V + c;
+          const float v = (cols[c] + cols[LPR * V + c]) + (cols[2 * LPR * V + c] + cols[3 * LPR * V + c]);
+          if (e < C) {
+            if (p.part) part[k * C + e] = v;
+            else if (k ? p.db : p.dw) store_as(k ? p.db : p.dw, p.wcode, e, v);
+          }
+        }
+      } else {
+        const int e = (l + i * LPR) * V;
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (j < n[i]) {
+            if (p.part) part[k * C + e + j] = t[j];
+            else if (k ? p.db : p.dw) store_as(k ? p.db : p.dw, p.wcode, e + j, t[j]);
+          }
+      }
+    }
+}
+
+// out0 / out1[c] = sum over the nblk partial rows of part[blk][0 / 1][c] (a fixed order: the slices of a column in order, then the
+// slices' sums in order).  32 columns x 8 slices a block.
+__global__ __launch_bounds__(NTHR) void column_reduce_kernel(const float* part, void* o0, void* o1, int code0, int code1, int nblk, int C, int width) {
+  __shared__ float lds[8][33];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + tx;
+  float s = 0.0f;
+  if (c < width) {
+#pragma unroll 4
+    for (int b = ty; b < nblk; b += 8) s += part[(long)b * width + c];
+  }
+  lds[ty][tx] = s;
+  __syncthreads();
+  if (ty == 0 && c < width) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k) s += lds[k][tx];
+    if (c < C) { if (o0) store_as(o0, code0, c, s); }
+    else if (o1) store_as(o1, code1, c - C, s);
+  }
+}
+
+// lanes per row and vectors per lane for a row of `chunks` vectors: the fewest lanes that hold it in at most 5 vectors each (more
+// rows per wave, fewer steps per sum), then the fewest vectors of the forms that are built
+struct Shape { int lpr, nv; };
+Shape pick(int chunks) {
+  for (int lpr = 8; lpr <= 64; lpr *= 2)
+    if (chunks <= 5 * lpr) return {lpr, chunks <= 2 * lpr ? 2 : chunks <= 3 * lpr ? 3 : 5};
+  return {256, chunks <= 2 * 256 ? 2 : chunks <= 4 * 256 ? 4 : 8};
+}
+
+#define HI3D_NORM_SHAPES(LAUNCH)                                                                                  \
+  if (s.lpr == 8) { if (s.nv == 2) LAUNCH(8, 2); else if (s.nv == 3) LAUNCH(8, 3); else LAUNCH(8, 5); }           \
+  else if (s.lpr == 16) { if (s.nv == 3) LAUNCH(16, 3); else if (s.nv == 2) LAUNCH(16, 2); else LAUNCH(16, 5); }  \
+  else if (s.lpr == 32) { if (s.nv == 3) LAUNCH(32, 3); else if (s.nv == 2) LAUNCH(32, 2); else LAUNCH(32, 5); }  \
+  else if (s.lpr == 64) { if (s.nv == 3) LAUNCH(64, 3); else if (s.nv == 2) LAUNCH(64, 2); else LAUNCH(64, 5); }  \
+  else { if (s.nv == 2) LAUNCH(256, 2); else if (s.nv == 4) LAUNCH(256, 4); else LAUNCH(256, (Elem<T>::VEC == 8 ? 4 : 8)); }   /* 8192 wide */
+
+constexpr int FWD_BLOCKS = 2048;      // 8 blocks of 4 waves a CU
+constexpr int BWD_BLOCKS = 512;       // 2 a CU: each writes 8 C bytes of partial sums
+
+long blocks_for(long R, int lpr, long most) {
+  const long rpb = NTHR / lpr, n = (R + rpb - 1) / rpb;
+  return n < most ? n : most;
+}
+
+template <typename T>
+int launch_fwd(const NormFwdParams& p, hipStream_t st) {
+  const Shape s = pick((p.C + Elem<T>::VEC - 1) / Elem<T>::VEC);
+  const dim3 grid((unsigned)blocks_for(p.R, s.lpr, FWD_BLOCKS));
+#define HI3D_L(LPR, NV)                                                                                               \
+  do {                                                                                                                \
+    if (p.r) hipLaunchKernelGGL((norm_fwd_kernel<T, LPR, NV, true>), grid, dim3(NTHR), 0, st, p);                     \
+    else hipLaunchKernelGGL((norm_fwd_kernel<T, LPR, NV, false>), grid, dim3(NTHR), 0, st, p);                        \
+  } while (0)
+  HI3D_NORM_SHAPES(HI3D_L)
+#undef HI3D_L
+  HI3D_LAUNCH_CHECK();
+  return 0;
+}
+
+template <typename T>
+int launch_bwd(const NormBwdParams& p, int nblk, hipStream_t st) {
+  const Shape s = pick((p.C + Elem<T>::VEC - 1) / Elem<T>::VEC);
+  const dim3 grid((unsigned)nblk);
+#define HI3D_L(LPR, NV) hipLaunchKernelGGL((norm_bwd_kernel<T, LPR, NV>), grid, dim3(NTHR), 0, st, p)
+  HI3D_NORM_SHAPES(HI3D_L)
+#undef HI3D_L
+  HI3D_LAUNCH_CHECK();
+  return 0;
+}
+
+int bwd_blocks(long R, int C, int dtype) {
+  const int vec = dtype == HI3D_F32 ? 4 : 8;
+  return (int)blocks_for(R, pick((C + vec - 1) / vec).lpr, BWD_BLOCKS);
+}
+
+int bad_sizes(const char* what, long R, int C, int dtype, int wcode) {
+  if (!hi3d_known_dtype(dtype) || !hi3d_known_dtype(wcode)) HI3D_FAIL(HI3D_EINVAL, "layernorm training: unknown element type");
+  if (R < 0 || C <= 0) HI3D_FAIL(HI3D_EINVAL, "layernorm training: negative row count or width < 1");
+  if (C > HI3D_NORM_MAX_WIDTH) HI3D_FAIL(HI3D_ESHAPE, "layernorm training: width over 8192");
+  return 0;
+}
+
+}  // namespace
+
+int hi3d_column_reduce(const float* part, void* o0, void* o1, int code0, int code1, int nblk, int C, int width, hipStream_t st) {
+  hipLaunchKernelGGL(column_reduce_kernel, dim3((width + 31) / 32), dim3(NTHR), 0, st, part, o0, o1, code0, code1, nblk, C, width);
+  HI3D_LAUNCH_CHECK();
+  return 0;
+}
+
+extern "C" int hi3d_layernorm_fwd(const void* x, const void* residual, const void* weight, const void* bias, void* y, void* z, float* mean,
+                                  float* rstd, int64_t R, int32_t C, int64_t ldx, int64_t ldr, int32_t dtype, int32_t wdtype, float eps, void* stream) {
+  if (const int rc = bad_sizes("fwd", R, C, dtype, wdtype)) return rc;
+  if (!(eps >= 0.0f) || eps > 3.0e38f) HI3D_FAIL(HI3D_EINVAL, "layernorm_fwd: eps must be finite and not negative");
+  if (R == 0) return 0;
+  if (!x || !y || !mean || !rstd || (residual && !z)) HI3D_FAIL(HI3D_EINVAL, "layernorm_fwd: null pointer");
+  if ((ldx < C && R > 1) || (residual && ldr < C && R > 1)) HI3D_FAIL(HI3D_EINVAL, "layernorm_fwd: row pitch below the width");
+  const NormFwdParams p = {x, residual, weight, bias, y, z, mean, rstd, (long)R, (long)ldx, (long)ldr, C, wdtype, eps};
+  if (dtype == HI3D_F32) return launch_fwd<float>(p, (hipStream_t)stream);
+  return dtype == HI3D_BF16 ? launch_fwd<bf16_t>(p, (hipStream_t)stream) : launch_fwd<half_t>(p, (hipStream_t)stream);
+}
+
+extern "C" int64_t hi3d_layernorm_bwd_workspace_floats(int64_t R, int32_t C, int32_t dtype) {
+  if (R <= 0 || C <= 0 || C > HI3D_NORM_MAX_WIDTH || !hi3d_known_dtype(dtype)) return 0;
+  const int n = bwd_blocks((long)R, C, dtype);
+  return n > 1 ? (int64_t)n * 2 * C : 0;
+}
+
+extern "C" int hi3d_layernorm_bwd(const void* dy, const void* z, const void* dz, const void* weight, const float* mean, const float* rstd, void* dx,
+                                  void* dweight, void* dbias, float* ws, int64_t R, int32_t C, int64_t lddy, int64_t ldz, int64_t lddz, int32_t dtype,
+                                  int32_t wdtype, void* stream) {
+  if (const int rc = bad_sizes("bwd", R, C, dtype, wdtype)) return rc;
+  const hipStream_t st = (hipStream_t)stream;
+  if (R == 0) return (dweight || dbias) ? hi3d_column_reduce(nullptr, dweight, dbias, wdtype, wdtype, 0, C, 2 * C, st) : 0;   // sums of nothing
+  if (!dy || !z || !mean || !rstd || !dx) HI3D_FAIL(HI3D_EINVAL, "layernorm_bwd: null pointer");
+  if (R > 1 && (lddy < C || ldz < C || (dz && lddz < C))) HI3D_FAIL(HI3D_EINVAL, "layernorm_bwd: row pitch below the width");
+  const int nblk = bwd_blocks((long)R, C, dtype), want = (dweight || dbias) ? 1 : 0;
+  if (want && nblk > 1 && !ws) HI3D_FAIL(HI3D_EINVAL, "layernorm_bwd: workspace required (hi3d_layernorm_bwd_workspace_floats)");
+  const NormBwdParams p = {dy, z, dz, weight, mean, rstd, dx, nblk > 1 ? ws : nullptr, dweight, dbias, (long)R, (long)lddy, (long)ldz, (long)lddz, C, wdtype, want};
+  const int rc = dtype == HI3D_F32 ? launch_bwd<float>(p, nblk, st) : dtype == HI3D_BF16 ? launch_bwd<bf16_t>(p, nblk, st) : launch_bwd<half_t>(p, nblk, st);
+  if (rc || !want || nblk == 1) return rc;
+  return hi3d_column_reduce(ws, dweight, dbias, wdtype, wdtype, nblk, C, 2 * C, st);
+}

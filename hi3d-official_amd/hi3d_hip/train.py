@@ -1,0 +1,151 @@
+"""Training with the gfx950 kernels: operators with gradients, and the optimiser.
+
+The sampler's operators (hi3d_hip.ops, torch.ops.hi3d.layernorm / linear) have no gradients.  These do, for a module tree that is
+trained through the operator binding:
+
+    from hi3d_hip import train
+    y = train.layer_norm(x, weight, bias)                       # nn.LayerNorm
+    y, z = train.layer_norm(x, weight, bias, residual=r)        # z = x + r, y = LayerNorm(z)
+    opt = train.AdamW(model.parameters(), lr=1e-5)              # torch.optim.AdamW
+
+`AdamW` is a torch.optim.Optimizer and so a `target:` of the reference's YAML (`optimizer_config`).  Underneath are
+torch.ops.hi3d.layernorm_fwd / add_layernorm_fwd / layernorm_bwd / adamw_, which may be called by themselves: a step that is
+captured into a HIP graph calls these, since a captured autograd backward shares its leaves' gradient nodes -- and the
+stream they were made on -- with any eager graph of the same leaves that is still alive.
+"""
+import torch
+
+from . import lib as _l
+from . import torch_ops
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, eps):
+        ns = torch_ops.load()
+        ctx.set_materialize_grads(False)
+        if residual is None:
+            y, mean, rstd = ns.layernorm_fwd(x, weight, bias, eps)
+            ctx.save_for_backward(x, mean, rstd, weight, bias)
+            return y
+        y, z, mean, rstd = ns.add_layernorm_fwd(x, residual, weight, bias, eps)
+        ctx.save_for_backward(z, mean, rstd, weight, bias)
+        return y, z
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dz=None):
+        z, mean, rstd, weight, bias = ctx.saved_tensors
+        if dy is None:                               # nothing reads y: the gradient passes through the sum alone
+            return dz, dz, None, None, None
+        dx, dw, db = torch_ops.load().layernorm_bwd(dy, z, mean, rstd, weight, bias, dz)
+        return dx, dx if ctx.needs_input_grad[1] else None, dw, db, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
+    """LayerNorm over x's last dimension, differentiable: y, or (y, x + residual) where a residual of x's shape and type is given.
+    x: fp32, bf16 or fp16, any strides; weight, bias: [width] of one of these types, or None; width up to 8192.  The sum is
+    rounded to x's type before it is normalised (it is what the next layer reads); statistics and sums are fp32."""
+    return _LayerNorm.apply(x, residual, weight, bias, float(eps))
+
+
+class AdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW's update for all tensors of a group in one launch per 72 of them (torch.ops.hi3d.adamw_).
+
+    Parameters fp32, bf16 or fp16 on one GPU, dense in memory; moments are fp32 whatever the parameter's type.
+    working_dtype (torch.bfloat16 / torch.float16): fp32 parameters keep a copy in that type which every step rewrites -- the
+    weights the forward pass reads, `working_copy(p)`.
+    capturable: step count on the device (per group: each of its parameters then needs a gradient at every step), so that step() can be
+    captured into a HIP graph; `lr` may then be a one-element fp32 device tensor.  torch.amp.GradScaler's scale and
+    overflow flag are read on the device in this mode.
+    """
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, working_dtype=None, capturable=False):
+        if torch.is_tensor(lr):
+            if not capturable:
+                raise ValueError("lr as a tensor needs capturable=True")
+        elif not lr >= 0.0:
+            raise ValueError(f"invalid learning rate: {lr}")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+            raise ValueError(f"invalid betas: {betas}")
+        if not eps >= 0.0 or not weight_decay >= 0.0:
+            raise ValueError(f"invalid eps or weight_decay: {eps}, {weight_decay}")
+        if working_dtype not in (None, torch.bfloat16, torch.float16):
+            raise ValueError(f"working_dtype must be torch.bfloat16 or torch.float16, not {working_dtype}")
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, working_dtype=working_dtype,
+                                      capturable=capturable, step_t=None))
+        self._step_supports_amp_scaling = all(g["capturable"] for g in self.param_groups)
+
+    def working_copy(self, p):
+        """The 16-bit copy of parameter p that step() keeps (its value before the first step: p rounded)."""
+        return self._state_of(p, self._group_of(p))["copy"]
+
+    def _group_of(self, p):
+        for g in self.param_groups:
+            if any(q is p for q in g["params"]):
+                if g["working_dtype"] is None:
+                    raise ValueError("this parameter's group has no working_dtype")
+                return g
+        raise KeyError("not a parameter of this optimiser")
+
+    def _state_of(self, p, group):
+        s = self.state[p]
+        if "exp_avg" not in s:
+            s["step"] = 0
+            s["exp_avg"] = torch.zeros_like(p, dtype=torch.float32)
+            s["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32)
+            if group["working_dtype"] is not None:
+                if p.dtype != torch.float32:
+                    raise _l.Hi3dError("a working copy is kept of fp32 parameters only")
+                s["copy"] = p.detach().to(group["working_dtype"])
+        return s
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        ns = torch_ops.load()
+        scale, found_inf = getattr(self, "grad_scale", None), getattr(self, "found_inf", None)
+        for group in self.param_groups:
+            with_grad = [p for p in group["params"] if p.grad is not None]
+            if group["capturable"] and with_grad and len(with_grad) < len(group["params"]):
+                raise _l.Hi3dError("capturable: every parameter of the group needs a gradient at every step")
+            by_step = {}                                    # (one list, unless some parameters had no gradient at earlier steps)
+            for p in with_grad:
+                g = p.grad
+                if g.is_sparse:
+                    raise _l.Hi3dError("sparse gradients are not supported")
+                if g.stride() != p.stride():
+                    g = torch.empty_like(p, dtype=g.dtype).copy_(g)
+                s = self._state_of(p, group)
+                if not group["capturable"]:
+                    s["step"] += 1
+                lists = by_step.setdefault((p.device, s["step"]), ([], [], [], [], []))
+                for to, t in zip(lists, (p, g, s["exp_avg"], s["exp_avg_sq"], s.get("copy"))):
+                    if t is not None:
+                        to.append(t)
+            b1, b2 = group["betas"]
+            for (dev, step), lists in by_step.items():
+                lr_t = step_t = None
+                if group["capturable"]:
+                    if group["step_t"] is None:
+                        group["step_t"] = torch.zeros(1, device=dev)
+                    step_t, lr_t = group["step_t"], group["lr"] if torch.is_tensor(group["lr"]) else None
+                ns.adamw_(*lists, 0.0 if lr_t is not None else float(group["lr"]), b1, b2, group["eps"], group["weight_decay"], max(step, 1), step_t, lr_t,
+                          scale if step_t is not None else None, found_inf if step_t is not None else None)
+        return loss
+
+    def load_state_dict(self, state_dict):
+        """As torch's, but the moments and copies keep their own types (torch casts a state to its parameter's type)."""
+        super().load_state_dict(state_dict)
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
+            for k, v in state_dict["state"].get(i, {}).items():
+                if torch.is_tensor(v):
+                    self.state[p][k] = torch.empty_like(p, dtype=v.dtype).copy_(v)
+        for g in self.param_groups:
+            if g["step_t"] is not None and g["params"]:
+                g["step_t"] = g["step_t"].detach().clone().to(g["params"][0].device)
+        self._step_supports_amp_scaling = all(g["capturable"] for g in self.param_groups)

@@ -320,6 +320,47 @@ int hi3d_layernorm(const void* x, void* y, void* sum_out, const float* gamma,
                    const float* beta, const float* addvec, int32_t rows_per_group,
                    int32_t R, int32_t C, float eps, void* stream);
 
+/* LayerNorm for training: beside hi3d_layernorm (the sampler's form: bf16, widths that are multiples of 8), any of three
+ * element types, any width up to HI3D_NORM_MAX_WIDTH, rows at any pitch and any element alignment, and its gradients.
+ *   z = x (+ residual, rounded to x's type);  y = (z - mean) * rstd * weight + bias;  mean, rstd: fp32 [R]
+ * x, residual, y, z: `dtype`; weight, bias (either may be NULL): `wdtype`.  z is written only where there is a residual (else
+ * z may be NULL); y, z are dense [R][C].  Nothing overlaps.
+ *   dx = rstd * (weight dy - mean(weight dy) - h mean(weight dy h)) (+ dz),  h = (z - mean) * rstd
+ *   dweight = sum_r dy h,  dbias = sum_r dy       (wdtype; fixed order of the sums: the same bits every time)
+ * dz (may be NULL): the gradient that arrives at z by its other reader.  dx, the gradient of x and of the residual alike, is
+ * dense [R][C].  dweight / dbias may be NULL.  ws: hi3d_layernorm_bwd_workspace_floats(R, C, dtype) floats (NULL where that is 0).
+ * R = 0 writes zero gradients of weight and bias and nothing else.                                    */
+#define HI3D_F32 0
+#define HI3D_BF16 1
+#define HI3D_F16 2
+#define HI3D_NORM_MAX_WIDTH 8192
+int hi3d_layernorm_fwd(const void* x, const void* residual, const void* weight, const void* bias, void* y, void* z,
+                       float* mean, float* rstd, int64_t R, int32_t C, int64_t ldx, int64_t ldr, int32_t dtype,
+                       int32_t wdtype, float eps, void* stream);
+int64_t hi3d_layernorm_bwd_workspace_floats(int64_t R, int32_t C, int32_t dtype);
+int hi3d_layernorm_bwd(const void* dy, const void* z, const void* dz, const void* weight, const float* mean,
+                       const float* rstd, void* dx, void* dweight, void* dbias, float* ws, int64_t R, int32_t C,
+                       int64_t lddy, int64_t ldz, int64_t lddz, int32_t dtype, int32_t wdtype, void* stream);
+
+/* One AdamW step over n tensors (decoupled weight decay; 32-bit moments), in place:
+ *   m <- beta1 m + (1 - beta1) g';  v <- beta2 v + (1 - beta2) g'^2;  p <- p * shrink - step_size * m / (sqrt(v) * inv_root + eps)
+ * with g' = g * grad_scale, shrink = 1 - lr * weight_decay, step_size = lr / (1 - beta1^t), inv_root = 1 / sqrt(1 - beta2^t).
+ * p: pdtype, g: gdtype, m / v: fp32, copy (may be NULL): copy_dtype (HI3D_BF16 / HI3D_F16), p rounded once more.  Every tensor is n
+ * dense elements at any element alignment (n = 0: nothing).  The table is read on the host during the call.  Tensors that are written overlap
+ * nothing else of the call.  coefs_dev (may be NULL): hi3d_adamw_coefs' output replaces shrink, step_size, inv_root and grad_scale of *c.
+ *
+ * hi3d_adamw_coefs: the four (and a flag) for a step whose count lives on the device: *step += 1, unless *found_inf (may be NULL) is
+ * not zero -- then the count stays and hi3d_adamw_step with this output changes nothing.  out: HI3D_ADAMW_COEFS floats.  lr_dev
+ * replaces lr; grad_scale is the loss scale, by which gradients are divided (either may be NULL).       */
+typedef struct { void* p; const void* g; float* m; float* v; void* copy; int64_t n; } hi3d_adamw_tensor;
+typedef struct { float shrink, step_size, inv_root, grad_scale, beta1, one_minus_beta1, beta2, one_minus_beta2, eps; } hi3d_adamw_coefs_t;
+#define HI3D_ADAMW_SKIP 4
+#define HI3D_ADAMW_COEFS 8
+int hi3d_adamw_coefs(float* out, float* step, const float* lr_dev, const float* grad_scale, const float* found_inf,
+                     double lr, double beta1, double beta2, double weight_decay, void* stream);
+int hi3d_adamw_step(const hi3d_adamw_tensor* t, int32_t n, int32_t pdtype, int32_t gdtype, int32_t copy_dtype,
+                    const hi3d_adamw_coefs_t* c, const float* coefs_dev, void* stream);
+
 /* ------------------------------------------------------------------------ */
 /* Layout / elementwise                                                      */
 /* ------------------------------------------------------------------------ */

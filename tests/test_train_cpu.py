@@ -1,0 +1,69 @@
+"""The training kernels' entry points without a GPU: what they refuse before anything is launched, and that they are there."""
+import ctypes as C
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from hi3d_hip import lib as l
+    return l.load()
+
+
+BAD_TYPE, F32, BF16 = 9, 0, 1
+P = 4096          # a pointer that is never followed
+
+
+def norm_fwd(lib, **k):
+    a = dict(x=P, r=0, w=P, b=P, y=P, z=0, mean=P, rstd=P, R=4, C=8, ldx=8, ldr=0, dt=F32, wdt=F32, eps=1e-5) | k
+    return lib.hi3d_layernorm_fwd(a["x"], a["r"], a["w"], a["b"], a["y"], a["z"], a["mean"], a["rstd"], a["R"], a["C"], a["ldx"], a["ldr"], a["dt"], a["wdt"], a["eps"], 0)
+
+
+@pytest.mark.parametrize("k", [dict(x=0), dict(y=0), dict(mean=0), dict(rstd=0), dict(r=P), dict(R=-1), dict(C=0), dict(C=8193), dict(dt=BAD_TYPE), dict(wdt=BAD_TYPE),
+                               dict(eps=-1.0), dict(eps=float("nan")), dict(eps=float("inf")), dict(ldx=7), dict(r=P, z=P, ldr=7)])
+def test_layernorm_fwd_refuses(lib, k):
+    assert norm_fwd(lib, **k) < 0 and lib.hi3d_last_error()
+
+
+def test_layernorm_of_no_rows_is_nothing(lib):
+    assert norm_fwd(lib, R=0, x=0, y=0, mean=0, rstd=0) == 0
+    assert lib.hi3d_layernorm_bwd(*[0] * 10, 0, 8, 8, 8, 8, F32, F32, 0) == 0
+
+
+def test_layernorm_bwd_refuses(lib):
+    def bwd(**k):
+        a = dict(dy=P, z=P, dz=0, w=P, mean=P, rstd=P, dx=P, dw=P, db=P, ws=P, R=100000, C=8, lddy=8, ldz=8, lddz=8, dt=F32, wdt=F32) | k
+        return lib.hi3d_layernorm_bwd(*[a[n] for n in ("dy", "z", "dz", "w", "mean", "rstd", "dx", "dw", "db", "ws", "R", "C", "lddy", "ldz", "lddz", "dt", "wdt")], 0)
+    for k in (dict(dy=0), dict(z=0), dict(mean=0), dict(rstd=0), dict(dx=0), dict(ws=0), dict(R=-1), dict(C=0), dict(C=8193), dict(dt=BAD_TYPE), dict(wdt=-1),
+              dict(lddy=7), dict(ldz=0), dict(dz=P, lddz=7)):
+        assert bwd(**k) < 0, k
+    assert lib.hi3d_layernorm_bwd_workspace_floats(1, 8, F32) == 0 and lib.hi3d_layernorm_bwd_workspace_floats(-1, 8, F32) == 0
+    assert lib.hi3d_layernorm_bwd_workspace_floats(1 << 40, 640, BF16) == 512 * 2 * 640
+
+
+def test_adamw_refuses(lib):
+    class T(C.Structure):
+        _fields_ = [("p", C.c_void_p), ("g", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p), ("copy", C.c_void_p), ("n", C.c_int64)]
+    coefs = (C.c_float * 9)()
+    step = lambda t, n, pd=F32, gd=F32, cd=BF16, c=coefs: lib.hi3d_adamw_step(C.addressof(t) if t is not None else 0, n, pd, gd, cd, C.addressof(c) if c is not None else 0, 0, 0)
+    ok = T(P, P, P, P, 0, 0)
+    assert step(ok, 1) == 0 and step(None, 0) == 0                    # no elements, no tensors: nothing is launched
+    for t, n, kw in ((None, 1, {}), (ok, -1, {}), (ok, 1, dict(pd=BAD_TYPE)), (ok, 1, dict(gd=BAD_TYPE)), (ok, 1, dict(cd=F32)), (ok, 1, dict(c=None)),
+                     (T(0, P, P, P, 0, 4), 1, {}), (T(P, 0, P, P, 0, 4), 1, {}), (T(P, P, 0, P, 0, 4), 1, {}), (T(P, P, P, 0, 0, 4), 1, {}), (T(P, P, P, P, 0, -4), 1, {})):
+        assert step(t, n, **kw) < 0
+    assert lib.hi3d_adamw_coefs(0, P, 0, 0, 0, 1.0, 0.9, 0.99, 0.0, 0) < 0 and lib.hi3d_adamw_coefs(P, 0, 0, 0, 0, 1.0, 0.9, 0.99, 0.0, 0) < 0
+
+
+def test_cpu_tensors_are_refused():
+    from hi3d_hip import torch_ops, train
+    ns = torch_ops.load()
+    x = torch.zeros(2, 4)
+    for f in (lambda: ns.layernorm_fwd(x, None, None, 1e-5), lambda: ns.add_layernorm_fwd(x, x, None, None, 1e-5), lambda: train.layer_norm(x),
+              lambda: ns.adamw_([x], [x], [x], [x], [], 0.1, 0.9, 0.99, 1e-8, 0.0, 1, None, None, None, None)):
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            f()
+    opt = train.AdamW([torch.nn.Parameter(x)])
+    opt.param_groups[0]["params"][0].grad = x.clone()
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        opt.step()
