@@ -84,17 +84,16 @@ __global__ __launch_bounds__(THR) void adamw_kernel(const AdamwArgs a) {
 }
 
 // the coefficients of a step whose count (and learning rate, loss scale, overflow flag) live in device memory
-__global__ void adamw_coefs_kernel(float* out, float* step, const float* lr_dev, const float* scale, const float* found_inf, double lr, double b1, double b2,
-                                   double wd) {
+__global__ void adamw_coefs_kernel(float* out, float* step, const float* lr_dev, const float* scale, const float* found_inf, hi3d_adamw_rates r) {
   const bool skip = found_inf && *found_inf != 0.0f;
   out[HI3D_ADAMW_SKIP] = skip ? 1.0f : 0.0f;
   if (skip) return;
   const float t = *step + 1.0f;
   *step = t;
-  if (lr_dev) lr = (double)*lr_dev;
-  out[0] = (float)(1.0 - lr * wd);
-  out[1] = (float)(lr / (1.0 - pow(b1, (double)t)));
-  out[2] = (float)(1.0 / sqrt(1.0 - pow(b2, (double)t)));
+  const double lr = lr_dev ? (double)*lr_dev : r.lr;
+  out[0] = (float)(1.0 - lr * r.weight_decay);
+  out[1] = (float)(lr / (1.0 - pow(r.beta1, (double)t)));
+  out[2] = (float)(1.0 / sqrt(1.0 - pow(r.beta2, (double)t)));
   out[3] = scale ? (float)(1.0 / (double)*scale) : 1.0f;
 }
 
@@ -113,10 +112,10 @@ int launch_g(const AdamwArgs& a, unsigned blocks, int gdtype, int copy_dtype, hi
 
 }  // namespace
 
-extern "C" int hi3d_adamw_coefs(float* out, float* step, const float* lr_dev, const float* grad_scale, const float* found_inf, double lr, double beta1,
-                                double beta2, double weight_decay, void* stream) {
-  if (!out || !step) HI3D_FAIL(HI3D_EINVAL, "adamw_coefs: null pointer");
-  hipLaunchKernelGGL(adamw_coefs_kernel, dim3(1), dim3(1), 0, (hipStream_t)stream, out, step, lr_dev, grad_scale, found_inf, lr, beta1, beta2, weight_decay);
+extern "C" int hi3d_adamw_coefs(float* out, float* step, const float* lr_dev, const float* grad_scale, const float* found_inf,
+                                const hi3d_adamw_rates* rates, void* stream) {
+  if (!out || !step || !rates) HI3D_FAIL(HI3D_EINVAL, "adamw_coefs: null pointer");
+  hipLaunchKernelGGL(adamw_coefs_kernel, dim3(1), dim3(1), 0, (hipStream_t)stream, out, step, lr_dev, grad_scale, found_inf, *rates);
   HI3D_LAUNCH_CHECK();
   return 0;
 }

@@ -1,0 +1,636 @@
+// A linear layer with its epilogue, and its gradients:
+//
+//   z = x w^T + b        y = act(z) (+ residual)                       x [M, K]   w [N, K]   bf16 or fp16, products and sums fp32
+//   dz = dy act'(z)      dx = dz w      dw = dz^T x      db = sum over rows of dz
+//
+// Beside hi3d_gemm_bf16, whose operands are laid out once for the sampler (K a multiple of 64, both operands contiguous along the
+// contraction).  Here all three products read the tensors as a training step holds them: an operand is either contiguous along the
+// contraction (KC: x and w forward, dz for dx) or across it (KS: w for dx, both for dw), and a KS tile reaches the matrix instruction
+// through gfx950's transposing LDS read, so nothing is transposed in memory.
+#include "train_common.h"
+#include <type_traits>
+
+namespace {
+
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(8))) __bf16 bfx8;
+
+constexpr int BK = 64;
+
+// ---- activations ------------------------------------------------------------------------------------------------------------------
+// Phi(-a) = exp(-a^2 / 2) P(t), t = 1 / (1 + 0.3 a), a >= 0: P of degree 8 without constant term, fitted to the Mills ratio over
+// [0, 14] with least relative error, 1.5e-7 (4.6e-7 as evaluated in fp32) -- relative also where Phi is tiny, which an erf with an
+// absolute error would not give, and small enough for the fp32 sums of the bias' gradient.
+__device__ __forceinline__ void gauss(float x, float& cdf, float& bell) {
+  const float a = fabsf(x);
+  const float t = __builtin_amdgcn_rcpf(1.0f + 0.3f * a);
+  bell = __builtin_amdgcn_exp2f(a * a * -0.72134752044448170f);          // exp(-x^2 / 2)
+  float q = 0.03567480055634768f;
+  q = q * t - 0.15720318772763442f;
+  q = q * t + 0.20635367719077033f;
+  q = q * t - 0.053683791141534425f;
+  q = q * t + 0.12856169845786158f;
+  q = q * t + 0.09991347218457869f;
+  q = q * t + 0.12075395892859297f;
+  q = q * t + 0.11962929865929173f;
+  q = q * t * bell;
+  cdf = x < 0.0f ? q : 1.0f - q;
+}
+__device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.4426950408889634f)); }
+
+template <int N>
+__device__ __forceinline__ void activate(int act, float (&v)[N]) {
+  if (act == HI3D_ACT_GELU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) { float c, b; gauss(v[j], c, b); v[j] *= c; }
+  } else if (act == HI3D_ACT_SILU || act == HI3D_ACT_QUICK_GELU) {
+    const float s = act == HI3D_ACT_SILU ? 1.0f : 1.702f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] *= sigmoid(s * v[j]);
+  } else if (act == HI3D_ACT_RELU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = v[j] < 0.0f ? 0.0f : v[j];        // (keeps NaN)
+  }
+}
+// v[j] *= act'(z[j])
+template <int N>
+__device__ __forceinline__ void times_slope(int act, const float (&z)[N], float (&v)[N]) {
+  if (act == HI3D_ACT_GELU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) { float c, b; gauss(z[j], c, b); v[j] *= c + z[j] * b * 0.3989422804014327f; }
+  } else if (act == HI3D_ACT_SILU || act == HI3D_ACT_QUICK_GELU) {
+    const float s = act == HI3D_ACT_SILU ? 1.0f : 1.702f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) { const float g = sigmoid(s * z[j]); v[j] *= g * (1.0f + s * z[j] * (1.0f - g)); }
+  } else if (act == HI3D_ACT_RELU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = z[j] <= 0.0f ? 0.0f : v[j];
+  }
+}
+
+// ---- the epilogue of 8 consecutive columns of a row (the first `n` of them exist) ---------------------------------------------------
+struct Epilogue {
+  const void* bias; const void* res; void* y; void* z;
+  long ldr, ldo;
+  int bcode, act;
+};
+template <typename T>
+__device__ __forceinline__ void finish(const Epilogue& e, long m, int c, int n, float (&v)[8]) {
+  if (e.bias) {
+    float b[8];
+    load_vec_as(e.bias, e.bcode, c, n, b);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += b[j];
+  }
+  if (e.z) store_some((T*)e.z + m * e.ldo + c, n, v);
+  activate(e.act, v);
+  if (e.res) {
+    Pack<T, 8> k;
+    float r[8];
+    fetch((const T*)e.res + m * e.ldr + c, n, k);
+    unpack(k, r);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += r[j];
+  }
+  store_some((T*)e.y + m * e.ldo + c, n, v);
+}
+
+// ---- the product ------------------------------------------------------------------------------------------------------------------
+// out[M, N] = A B over the contraction of length K.  A is [M][K] (KC) or [K][M] (KS), B is [N][K] (KC) or [K][N] (KS); rows at a pitch
+// that is a multiple of 8 elements, 16-byte aligned; a row of KC holds zeros from K up to the next multiple of 8.
+struct MatParams {
+  const char* A; const char* B;
+  float* part;            // split contraction: partial sums [split][M][N]; NULL: the epilogue below
+  Epilogue e;
+  long lda, ldb;
+  int M, N, K, nbm, nbn, splits, per;      // per: K steps of a split
+  int group;                               // m-tiles that are walked before n moves on
+};
+
+template <typename T> struct Mfma;
+template <> struct Mfma<bf16_t> {
+  static __device__ __forceinline__ f32x4 mul(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+};
+template <> struct Mfma<half_t> {
+  static __device__ __forceinline__ f32x4 mul(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+};
+
+__device__ __forceinline__ int swap23(int i) { return (i & ~12) | ((i & 4) << 1) | ((i & 8) >> 1); }
+
+// One operand's tile of R rows (columns of the output) x 64 of the contraction, 128 bytes x R of LDS, filled by LDS-DMA in pieces of 1 KiB
+// (8 LDS rows of 128 bytes; a piece's lanes land in order, so what an LDS slot holds is chosen by the address that its lane reads).
+//
+// KC: LDS row r is operand row r, its 16-byte chunk c stands in slot c ^ ((r >> 1) & 7): a fragment read (16 rows, one chunk each) takes every
+//     bank once.
+// KS: panels of 64 columns; LDS row p of a panel is contraction row swap23(p) (bits 2 and 3 exchanged), its 32-byte unit u (16 columns)
+//     stands at u ^ ((p >> 1) & 3).  A transposing read takes [4 k][16 columns] per 16 lanes; with lane group g at k = 8 g + 4 h, the 8 LDS
+//     rows that half a wave touches are consecutive and their units fall on 8 different eighths of the banks.
+template <bool KS, int R, int NW>
+struct Tile {
+  static constexpr int PIECES = R / 8 / NW;
+  static_assert(R % 64 == 0 && (R / 8) % NW == 0, "whole panels, whole pieces");
+  unsigned off[PIECES];
+  int chunk[PIECES];                      // KC: the lane's 8-element chunk of the K step
+  const char* base;
+  long ld;                                // bytes
+  int rows, cols, first;                  // KC: rows of the tile that exist, K rounded up to 8;  KS: K, the output's columns rounded up to 8; its first column
+
+  __device__ __forceinline__ void init(const char* p, long ld_el, int r0, int total, int K, int wave, int lane) {
+    ld = ld_el * 2;
+    if (!KS) { base = p + (long)r0 * ld; rows = min(R, total - r0); cols = (K + 7) & ~7; first = 0; }
+    else { base = p + (long)r0 * 2; rows = K; cols = (total + 7) & ~7; first = r0; }
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int q = wave * PIECES + i;
+      if (!KS) {
+        const int r = q * 8 + (lane >> 3);
+        chunk[i] = (lane & 7) ^ ((r >> 1) & 7);
+        off[i] = (unsigned)(r * (int)ld + chunk[i] * 16);
+      } else {
+        const int pos = (q & 7) * 8 + (lane >> 3), u = ((lane & 7) >> 1) ^ ((pos >> 1) & 3);
+        chunk[i] = 0;
+        off[i] = (unsigned)(swap23(pos) * (int)ld + ((q >> 3) * 64 + u * 16 + (lane & 1) * 8) * 2);
+      }
+    }
+  }
+  // K step `kt` of the contraction into the tile at `lds`; what lies outside the operand is zero (beyond the descriptor's range)
+  __device__ __forceinline__ void issue(int kt, char* lds, int wave) const {
+    const int k0 = kt * BK;
+    const char* b = base + (KS ? (long)k0 * ld : (long)k0 * 2);
+    const long valid = KS ? (long)(min(rows - k0, BK) - 1) * ld + (long)(cols - first) * 2 : (long)(rows - 1) * ld + (long)(cols - k0) * 2;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)b, 0, (int)(valid > 0x7ffffff0 ? 0x7ffffff0 : valid), 0x00020000);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      unsigned o = off[i];
+      if (!KS && k0 + chunk[i] * 8 >= cols) o = 0x80000000u;       // behind the end of a row: not the next row's data
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (LDS_AS void*)(lds + (wave * PIECES + i) * 1024), 16, o, 0, 0, 0);
+    }
+  }
+};
+
+// The fragments of a wave's 16 * CNT rows (from row `first`) of a tile, half KH of its contraction
+template <bool KS, int CNT>
+struct Frags {
+  int addr[KS ? CNT : 1];
+  int sw;
+  __device__ __forceinline__ void init(int first, int lane) {
+    const int fr = lane & 15, fg = lane >> 4;
+    if (!KS) { addr[0] = (first + fr) * 128; sw = (fr >> 1) & 7; }
+    else {
+      const int x = ((fg & 1) << 1) | (fr >> 3);
+#pragma unroll
+      for (int t = 0; t < CNT; ++t) {
+        const int u = first / 16 + t;
+        addr[t] = (u >> 2) * 8192 + (fg >> 1) * 2048 + (fg & 1) * 512 + (fr >> 2) * 128 + (((u & 3) ^ x) << 5) + (fr & 3) * 8;
+      }
+      sw = 0;
+    }
+  }
+  // The transposing reads are in inline assembly, wait included: as builtins they would be kept behind every LDS-DMA in flight.
+  template <int KH>
+  __device__ __forceinline__ void read(const char* lds, u32x4 (&f)[CNT], int lane) const {
+    if constexpr (!KS) {
+      const char* p = lds + addr[0] + (((KH * 4 + (lane >> 4)) ^ sw) << 4);
+#pragma unroll
+      for (int t = 0; t < CNT; ++t) f[t] = *(const u32x4*)(p + t * 2048);
+    } else {
+      const unsigned b = (unsigned)(__UINTPTR_TYPE__)(LDS_AS const char*)lds;
+#pragma unroll
+      for (int t = 0; t < CNT; t += (CNT == 5 ? 5 : 4)) {
+        if constexpr (CNT == 5) {
+          u32x2 l0, l1, l2, l3, l4, h0, h1, h2, h3, h4;
+          asm volatile("ds_read_b64_tr_b16 %0, %10 offset:%15\n\tds_read_b64_tr_b16 %5, %10 offset:%16\n\t"
+                       "ds_read_b64_tr_b16 %1, %11 offset:%15\n\tds_read_b64_tr_b16 %6, %11 offset:%16\n\t"
+                       "ds_read_b64_tr_b16 %2, %12 offset:%15\n\tds_read_b64_tr_b16 %7, %12 offset:%16\n\t"
+                       "ds_read_b64_tr_b16 %3, %13 offset:%15\n\tds_read_b64_tr_b16 %8, %13 offset:%16\n\t"
+                       "ds_read_b64_tr_b16 %4, %14 offset:%15\n\tds_read_b64_tr_b16 %9, %14 offset:%16\n\t"
+                       "s_waitcnt lgkmcnt(0)"
+                       : "=&v"(l0), "=&v"(l1), "=&v"(l2), "=&v"(l3), "=&v"(l4), "=&v"(h0), "=&v"(h1), "=&v"(h2), "=&v"(h3), "=&v"(h4)
+                       : "v"(b + addr[0]), "v"(b + addr[1]), "v"(b + addr[2]), "v"(b + addr[3]), "v"(b + addr[CNT - 1]), "n"(KH * 4096), "n"(KH * 4096 + 1024)
+                       : "memory");
+          f[0] = u32x4{l0[0], l0[1], h0[0], h0[1]};
+          f[1] = u32x4{l1[0], l1[1], h1[0], h1[1]};
+          f[2] = u32x4{l2[0], l2[1], h2[0], h2[1]};
+          f[3] = u32x4{l3[0], l3[1], h3[0], h3[1]};
+          f[CNT - 1] = u32x4{l4[0], l4[1], h4[0], h4[1]};
+        } else {
+          u32x2 l0, l1, l2, l3, h0, h1, h2, h3;
+          asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %4, %8 offset:%13\n\t"
+                       "ds_read_b64_tr_b16 %1, %9 offset:%12\n\tds_read_b64_tr_b16 %5, %9 offset:%13\n\t"
+                       "ds_read_b64_tr_b16 %2, %10 offset:%12\n\tds_read_b64_tr_b16 %6, %10 offset:%13\n\t"
+                       "ds_read_b64_tr_b16 %3, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+                       "s_waitcnt lgkmcnt(0)"
+                       : "=&v"(l0), "=&v"(l1), "=&v"(l2), "=&v"(l3), "=&v"(h0), "=&v"(h1), "=&v"(h2), "=&v"(h3)
+                       : "v"(b + addr[t]), "v"(b + addr[t + 1]), "v"(b + addr[t + 2]), "v"(b + addr[t + 3]), "n"(KH * 4096), "n"(KH * 4096 + 1024)
+                       : "memory");
+          f[t] = u32x4{l0[0], l0[1], h0[0], h0[1]};
+          f[t + 1] = u32x4{l1[0], l1[1], h1[0], h1[1]};
+          f[t + 2] = u32x4{l2[0], l2[1], h2[0], h2[1]};
+          f[t + 3] = u32x4{l3[0], l3[1], h3[0], h3[1]};
+        }
+      }
+    }
+  }
+};
+
+// WM x WN waves, each 16 MT x 16 NT of the output; two tiles of the contraction in LDS, the next one on its way while one is used.
+// The weight-side fragment is the first operand of the matrix instruction, so that a lane holds 4 consecutive columns of one output row.
+template <typename T, bool AKS, bool BKS, int WM, int WN, int MT, int NT>
+__global__ __launch_bounds__(WM * WN * 64, 2) void mat_kernel(const MatParams p) {
+#if __HIP_DEVICE_COMPILE__
+  constexpr int NW = WM * WN, BM = 16 * MT * WM, BN = 16 * NT * WN;
+  constexpr int ABYTES = BM * 128, STAGE = (BM + BN) * 128;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = w / WN, wn = w % WN;
+
+  // block -> tile: neighbours in the order go to one XCD (its L2 keeps what they share); `group` m-tiles are walked for each n-tile
+  const int nblk = p.nbm * p.nbn;
+  int bid = blockIdx.x;
+  const int ks = bid / nblk;
+  bid -= ks * nblk;
+  const int q = nblk >> 3, r = nblk & 7, xcd = bid & 7, idx = bid >> 3;
+  const int lid = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + idx;
+  const int per = p.group * p.nbn, g = lid / per, rem = lid - g * per;
+  const int gh = min(p.group, p.nbm - g * p.group);
+  const int tn = rem / gh, tm = g * p.group + rem - tn * gh;
+  const int m0 = tm * BM, n0 = tn * BN;
+
+  Tile<AKS, BM, NW> ta;
+  Tile<BKS, BN, NW> tb;
+  ta.init(p.A, p.lda, m0, p.M, p.K, w, lane);
+  tb.init(p.B, p.ldb, n0, p.N, p.K, w, lane);
+  Frags<AKS, MT> fa;
+  Frags<BKS, NT> fb;
+  fa.init(wm * 16 * MT, lane);
+  fb.init(wn * 16 * NT, lane);
+
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  const int steps = (p.K + BK - 1) / BK, kb = ks * p.per, ke = min(steps, kb + p.per);
+  ta.issue(kb, smem, w);
+  tb.issue(kb, smem + ABYTES, w);
+  for (int kt = kb; kt < ke; ++kt) {
+    char* const s = smem + ((kt - kb) & 1) * STAGE;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();                              // tile kt is there, and everyone is done with the other one
+    if (kt + 1 < ke) {
+      char* const d = smem + ((kt + 1 - kb) & 1) * STAGE;
+      ta.issue(kt + 1, d, w);
+      tb.issue(kt + 1, d + ABYTES, w);
+    }
+    u32x4 a[MT], b[NT];
+    auto half = [&](auto kh) {
+      fa.template read<decltype(kh)::value>(s, a, lane);
+      fb.template read<decltype(kh)::value>(s + ABYTES, b, lane);
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = Mfma<T>::mul(b[j], a[i], acc[i][j]);
+    };
+    half(std::integral_constant<int, 0>{});
+    half(std::integral_constant<int, 1>{});
+  }
+  __syncthreads();                                // the tiles' LDS is free
+
+  // each wave turns its accumulators 16 rows at a time into whole rows, in a slab of its own, and finishes 8 columns a lane
+  constexpr int WCOLS = 16 * NT, ROW = WCOLS * 4 + 16, CPR = WCOLS / 8;
+  static_assert(NW * 16 * ROW <= 2 * STAGE, "slabs fit the tiles' LDS");
+  char* const slab = smem + w * 16 * ROW;
+  const int fr = lane & 15, fg = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) *(f32x4*)(slab + fr * ROW + (j * 16 + fg * 4) * 4) = acc[i][j];
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int t = 0; t < (16 * CPR + 63) / 64; ++t) {
+      const int c = t * 64 + lane, row = c / CPR, col = (c - row * CPR) * 8;
+      const long m = m0 + wm * 16 * MT + i * 16 + row;
+      const int n = n0 + wn * WCOLS + col;
+      if (c < 16 * CPR && m < p.M && n < p.N) {
+        const f32x4 lo = *(const f32x4*)(slab + row * ROW + col * 4), hi = *(const f32x4*)(slab + row * ROW + col * 4 + 16);
+        float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        if (p.part) store_some(p.part + ((long)ks * p.M + m) * p.N + n, p.N - n, v);
+        else finish<T>(p.e, m, n, p.N - n, v);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+#endif
+}
+
+// the partial sums of a split contraction, in the order of the splits, and the epilogue
+template <typename T>
+__global__ __launch_bounds__(256) void join_kernel(const float* part, Epilogue e, long M, int N, int splits) {
+  const int cpr = (N + 7) / 8;
+  for (long c = (long)blockIdx.x * 256 + threadIdx.x; c < M * cpr; c += (long)gridDim.x * 256) {
+    const long m = c / cpr;
+    const int n = (int)(c - m * cpr) * 8;
+    float v[8] = {};
+    for (int s = 0; s < splits; ++s) {
+      Pack<float, 8> k;
+      fetch(part + (s * M + m) * N + n, N - n, k);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += k.v[j];
+    }
+    finish<T>(e, m, n, N - n, v);
+  }
+}
+
+// rows of any pitch and alignment -> rows padded with zeros to a multiple of 8 elements, 16-byte aligned
+template <typename T>
+__global__ __launch_bounds__(256) void pad_kernel(const T* in, T* out, long rows, int cols, long ld) {
+  const int cpr = (cols + 7) / 8;
+  for (long c = (long)blockIdx.x * 256 + threadIdx.x; c < rows * cpr; c += (long)gridDim.x * 256) {
+    const long r = c / cpr;
+    const int e = (int)(c - r * cpr) * 8;
+    Pack<T, 8> k;
+    fetch(in + r * ld + e, cols - e, k);
+    *(Pack<T, 8>*)(out + r * (long)cpr * 8 + e) = k;
+  }
+}
+
+// dz = dy act'(z), rounded to the operands' type for the matrix instruction (its sums stay fp32), rows padded as above; and the column
+// sums of the unrounded dz, one row of partial sums per block row.  256 columns x 8 row lanes a block.
+struct SlopeParams {
+  const void* dy; const void* z; void* dz; float* part;
+  long M, lddy, ldz;
+  int N, act, rows;                        // rows: of a block
+};
+template <typename T>
+__global__ __launch_bounds__(256) void slope_kernel(const SlopeParams p) {
+  __shared__ float lds[8][256];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, c = blockIdx.x * 256 + tx * 8, n = p.N - c;
+  const long r0 = (long)blockIdx.y * p.rows, r1 = min(p.M, r0 + p.rows);
+  const long ldo = (p.N + 7) / 8 * 8;
+  float s[8] = {};
+  if (n > 0)
+    for (long r = r0 + ty; r < r1; r += 8) {
+      Pack<T, 8> ky, kz;
+      float v[8], z[8];
+      fetch((const T*)p.dy + r * p.lddy + c, n, ky);
+      if (p.act) fetch((const T*)p.z + r * p.ldz + c, n, kz);
+      unpack(ky, v);
+      if (p.act) {
+        unpack(kz, z);
+        times_slope(p.act, z, v);
+        if (n < 8) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = j < n ? v[j] : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] += v[j];
+      if (p.dz) store_some((T*)p.dz + r * ldo + c, 8, v);
+    }
+  if (!p.part) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) lds[ty][tx * 8 + j] = s[j];
+  __syncthreads();
+  const int col = blockIdx.x * 256 + threadIdx.x;
+  if (col < p.N) {
+    float t = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t += lds[k][threadIdx.x];
+    p.part[(long)blockIdx.y * p.N + col] = t;
+  }
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------------------------
+struct Config { int bm, bn, waves, slots; double step, fixed; };
+// step: us of one K step of a tile with the chip full, fixed: of a tile's start and end
+constexpr Config CONFIGS[] = {{256, 256, 8, 256, 1.75, 4.0}, {256, 320, 8, 256, 2.1, 4.5}, {128, 128, 4, 512, 1.1, 3.0}};
+constexpr int CUS = 256, MAX_SPLITS = 32;
+
+struct Plan { int cfg, splits, per; };
+// the tile and the split that the estimate above finds fastest
+Plan plan_of(long M, long N, long K) {
+  Plan best = {2, 1, 0};
+  double least = 1e300;
+  const long steps = (K + BK - 1) / BK;
+  for (int c = 0; c < 3; ++c) {
+    const Config& f = CONFIGS[c];
+    const long tiles = ((M + f.bm - 1) / f.bm) * ((N + f.bn - 1) / f.bn);
+    for (long s = 1; s <= MAX_SPLITS && s <= steps; ++s) {
+      const long per = (steps + s - 1) / s, splits = (steps + per - 1) / per;
+      if (splits != s) continue;
+      if (s > 1 && tiles * s > 4 * f.slots) break;
+      const double waves = (double)((tiles * s + f.slots - 1) / f.slots);
+      const double t = waves * (per * f.step + f.fixed) + (s > 1 ? 4.0 + (double)M * N * (8.0 * s + 4.0) / 4.0e6 : 0.0);
+      if (t < least) { least = t; best = {c, (int)s, (int)per}; }
+    }
+  }
+  return best;
+}
+
+long round256(long b) { return (b + 255) & ~255L; }
+long part_bytes(const Plan& p, long M, long N) { return p.splits > 1 ? round256(p.splits * M * N * 4) : 0; }
+
+template <typename T, bool AKS, bool BKS, int WM, int WN, int MT, int NT>
+int launch_cfg(const MatParams& p, hipStream_t st) {
+  constexpr int LDS = 2 * (16 * MT * WM + 16 * NT * WN) * 128;
+  static bool done[HI3D_MAX_DEVICES];
+  if (const int rc = hi3d_raise_lds_limit((const void*)mat_kernel<T, AKS, BKS, WM, WN, MT, NT>, LDS, done)) return rc;
+  hipLaunchKernelGGL((mat_kernel<T, AKS, BKS, WM, WN, MT, NT>), dim3((unsigned)(p.nbm * p.nbn * p.splits)), dim3(WM * WN * 64), LDS, st, p);
+  HI3D_LAUNCH_CHECK();
+  return 0;
+}
+unsigned grid_of(long items) { const long n = (items + 255) / 256; return (unsigned)(n < 1 ? 1 : n > 8192 ? 8192 : n); }
+
+template <typename T, bool AKS, bool BKS>
+int launch_mat(MatParams p, const Plan& plan, float* part, hipStream_t st) {
+  const Config& f = CONFIGS[plan.cfg];
+  p.nbm = (p.M + f.bm - 1) / f.bm; p.nbn = (p.N + f.bn - 1) / f.bn;
+  p.splits = plan.splits; p.per = plan.per; p.part = plan.splits > 1 ? part : nullptr;
+  p.group = 8;
+  int rc;
+  if (plan.cfg == 0) rc = launch_cfg<T, AKS, BKS, 2, 4, 8, 4>(p, st);
+  else if (plan.cfg == 1) rc = launch_cfg<T, AKS, BKS, 2, 4, 8, 5>(p, st);
+  else rc = launch_cfg<T, AKS, BKS, 2, 2, 4, 4>(p, st);
+  if (rc || plan.splits == 1) return rc;
+  hipLaunchKernelGGL((join_kernel<T>), dim3(grid_of((long)p.M * ((p.N + 7) / 8))), dim3(256), 0, st, (const float*)part, p.e, (long)p.M, p.N, plan.splits);
+  HI3D_LAUNCH_CHECK();
+  return 0;
+}
+
+// whether rows of `cols` elements can be read in place
+bool in_place(const void* p, long ld, long cols) { return !((uintptr_t)p & 15) && ld % 8 == 0 && cols % 8 == 0; }
+long padded_bytes(long rows, long cols) { return round256(rows * ((cols + 7) / 8 * 8) * 2); }
+
+template <typename T>
+int pad(const void* in, void* out, long rows, int cols, long ld, hipStream_t st) {
+  hipLaunchKernelGGL((pad_kernel<T>), dim3(grid_of(rows * ((cols + 7) / 8))), dim3(256), 0, st, (const T*)in, (T*)out, rows, cols, ld);
+  HI3D_LAUNCH_CHECK();
+  return 0;
+}
+
+struct Operand { const void* p; long ld; };
+// the operand itself, or -- where the kernel cannot read it in place -- a padded copy at *ws, which moves on
+template <typename T>
+int place(const void* p, long rows, int cols, long ld, char** ws, Operand* o, hipStream_t st) {
+  if (in_place(p, ld, cols)) { *o = {p, ld}; return 0; }
+  char* const to = *ws;
+  *ws += padded_bytes(rows, cols);
+  *o = {to, (cols + 7L) / 8 * 8};
+  return pad<T>(p, to, rows, cols, ld, st);
+}
+
+constexpr int SLOPE_BLOCKS = 2048;
+int slope_rows(long M, int N) {
+  const long cols = (N + 255) / 256, want = SLOPE_BLOCKS / cols > 0 ? SLOPE_BLOCKS / cols : 1;
+  long rows = (M + want - 1) / want;
+  rows = rows < 32 ? 32 : (rows + 7) / 8 * 8;
+  return (int)rows;
+}
+int slope_slices(long M, int N) { const int r = slope_rows(M, N); return (int)((M + r - 1) / r); }
+
+const char* bad_desc(const hi3d_linear_desc* d) {
+  if (!d) return "linear training: null descriptor";
+  if (d->M < 0 || d->N <= 0 || d->K <= 0) return "linear training: negative row count, or width < 1";
+  if (d->dtype != HI3D_BF16 && d->dtype != HI3D_F16) return "linear training: bf16 or fp16 operands";
+  if (d->bias_dtype != HI3D_F32 && d->bias_dtype != d->dtype) return "linear training: bias of fp32 or of the operands' type";
+  if (d->act < HI3D_ACT_NONE || d->act > HI3D_ACT_RELU) return "linear training: unknown activation";
+  return nullptr;
+}
+// tiles address their rows in 32 bits: 320 rows of 2 bytes an element
+bool too_big(const hi3d_linear_desc* d) {
+  const long most = 0x7ffffff0L / 640;
+  return d->M > 0x7fff0000L || d->N > most || d->K > most || d->N > 0x200000 || d->K > 0x200000 ||
+         (d->M > 1 && (d->ldx > most || d->lddy > most || d->ldz > (1L << 40) || d->ldr > (1L << 40))) || (d->N > 1 && d->ldw > most);
+}
+
+struct FwdNeeds { long x, w, part; Plan plan; };
+FwdNeeds fwd_needs(const hi3d_linear_desc* d) {
+  FwdNeeds n = {0, 0, 0, plan_of(d->M, d->N, d->K)};
+  if (!in_place(d->x, d->ldx, d->K)) n.x = padded_bytes(d->M, d->K);
+  if (!in_place(d->w, d->ldw, d->K)) n.w = padded_bytes(d->N, d->K);
+  n.part = part_bytes(n.plan, d->M, d->N);
+  return n;
+}
+struct BwdNeeds { long dz, x, w, part, cols; Plan dx, dw; };
+BwdNeeds bwd_needs(const hi3d_linear_desc* d) {
+  BwdNeeds n = {};
+  const bool copy = d->act != HI3D_ACT_NONE || !in_place(d->dy, d->lddy, d->N);
+  if ((d->dx || d->dw) && copy) n.dz = padded_bytes(d->M, d->N);
+  if (d->dw && !in_place(d->x, d->ldx, d->K)) n.x = padded_bytes(d->M, d->K);
+  if (d->dx && !in_place(d->w, d->ldw, d->K)) n.w = padded_bytes(d->N, d->K);
+  n.dx = plan_of(d->M, d->K, d->N);
+  n.dw = plan_of(d->N, d->K, d->M);
+  const long a = d->dx ? part_bytes(n.dx, d->M, d->K) : 0, b = d->dw ? part_bytes(n.dw, d->N, d->K) : 0;
+  n.part = a > b ? a : b;
+  if (d->db) n.cols = round256((long)slope_slices(d->M, d->N) * d->N * 4);
+  return n;
+}
+
+template <typename T>
+int fwd(const hi3d_linear_desc* d, hipStream_t st) {
+  const FwdNeeds n = fwd_needs(d);
+  char* ws = (char*)d->ws;
+  Operand x, w;
+  if (const int rc = place<T>(d->x, d->M, d->K, d->ldx, &ws, &x, st)) return rc;
+  if (const int rc = place<T>(d->w, d->N, d->K, d->ldw, &ws, &w, st)) return rc;
+  MatParams p = {};
+  p.A = (const char*)x.p; p.B = (const char*)w.p; p.lda = x.ld; p.ldb = w.ld;
+  p.M = (int)d->M; p.N = d->N; p.K = d->K;
+  p.e = {d->bias, d->residual, d->y, d->z, (long)d->ldr, (long)d->N, d->bias_dtype, d->act};
+  return launch_mat<T, false, false>(p, n.plan, (float*)ws, st);
+}
+
+template <typename T>
+int bwd(const hi3d_linear_desc* d, hipStream_t st) {
+  const BwdNeeds n = bwd_needs(d);
+  char* ws = (char*)d->ws;
+  Operand dz = {d->dy, (long)d->lddy};
+  void* to = nullptr;
+  if (n.dz) { to = ws; dz = {ws, (d->N + 7L) / 8 * 8}; ws += n.dz; }
+  if (n.dz || d->db) {
+    float* const cols = d->db ? (float*)ws : nullptr;
+    const int rows = slope_rows(d->M, d->N), slices = slope_slices(d->M, d->N);
+    const SlopeParams p = {d->dy, d->z, to, cols, (long)d->M, (long)d->lddy, (long)d->ldz, d->N, d->act, rows};
+    hipLaunchKernelGGL((slope_kernel<T>), dim3((d->N + 255) / 256, slices), dim3(256), 0, st, p);
+    HI3D_LAUNCH_CHECK();
+    if (d->db)
+      if (const int rc = hi3d_column_reduce(cols, d->db, nullptr, d->bias_dtype, 0, slices, d->N, d->N, st)) return rc;
+    ws += n.cols;
+  }
+  if (d->dx) {
+    Operand w;
+    if (const int rc = place<T>(d->w, d->N, d->K, d->ldw, &ws, &w, st)) return rc;
+    MatParams p = {};
+    p.A = (const char*)dz.p; p.B = (const char*)w.p; p.lda = dz.ld; p.ldb = w.ld;
+    p.M = (int)d->M; p.N = d->K; p.K = d->N;
+    p.e = {nullptr, nullptr, d->dx, nullptr, 0, (long)d->K, HI3D_F32, HI3D_ACT_NONE};
+    if (const int rc = launch_mat<T, false, true>(p, n.dx, (float*)((char*)d->ws + n.dz + n.cols + n.w + n.x), st)) return rc;
+  }
+  if (d->dw) {
+    Operand x;
+    if (const int rc = place<T>(d->x, d->M, d->K, d->ldx, &ws, &x, st)) return rc;
+    MatParams p = {};
+    p.A = (const char*)dz.p; p.B = (const char*)x.p; p.lda = dz.ld; p.ldb = x.ld;
+    p.M = d->N; p.N = d->K; p.K = (int)d->M;
+    p.e = {nullptr, nullptr, d->dw, nullptr, 0, (long)d->K, HI3D_F32, HI3D_ACT_NONE};
+    if (const int rc = launch_mat<T, true, true>(p, n.dw, (float*)((char*)d->ws + n.dz + n.cols + n.w + n.x), st)) return rc;
+  }
+  return 0;
+}
+
+}  // namespace
+
+extern "C" int64_t hi3d_linear_fwd_workspace_bytes(const hi3d_linear_desc* d) {
+  if (bad_desc(d) || too_big(d) || d->M == 0) return 0;
+  const FwdNeeds n = fwd_needs(d);
+  return n.x + n.w + n.part;
+}
+
+extern "C" int hi3d_linear_fwd(const hi3d_linear_desc* d, void* stream) {
+  if (const char* why = bad_desc(d)) HI3D_FAIL(HI3D_EINVAL, why);
+  if (too_big(d)) HI3D_FAIL(HI3D_ESHAPE, "linear_fwd: a size or pitch is over what a tile addresses");
+  if (d->M == 0) return 0;
+  if (!d->x || !d->w || !d->y) HI3D_FAIL(HI3D_EINVAL, "linear_fwd: null pointer");
+  if ((d->M > 1 && (d->ldx < d->K || (d->residual && d->ldr < d->N))) || (d->N > 1 && d->ldw < d->K)) HI3D_FAIL(HI3D_EINVAL, "linear_fwd: row pitch below the width");
+  const int64_t need = hi3d_linear_fwd_workspace_bytes(d);
+  if (need && (!d->ws || d->ws_bytes < need || ((uintptr_t)d->ws & 255))) HI3D_FAIL(HI3D_EINVAL, "linear_fwd: workspace missing, too small or not 256-byte aligned");
+  return d->dtype == HI3D_BF16 ? fwd<bf16_t>(d, (hipStream_t)stream) : fwd<half_t>(d, (hipStream_t)stream);
+}
+
+extern "C" int64_t hi3d_linear_bwd_workspace_bytes(const hi3d_linear_desc* d) {
+  if (bad_desc(d) || too_big(d) || d->M == 0) return 0;
+  const BwdNeeds n = bwd_needs(d);
+  return n.dz + n.x + n.w + n.cols + n.part;
+}
+
+extern "C" int hi3d_linear_bwd(const hi3d_linear_desc* d, void* stream) {
+  if (const char* why = bad_desc(d)) HI3D_FAIL(HI3D_EINVAL, why);
+  if (too_big(d)) HI3D_FAIL(HI3D_ESHAPE, "linear_bwd: a size or pitch is over what a tile addresses");
+  const hipStream_t st = (hipStream_t)stream;
+  if (d->M == 0) {                       // sums over no rows
+    if (d->db)
+      if (const int rc = hi3d_column_reduce(nullptr, d->db, nullptr, d->bias_dtype, 0, 0, d->N, d->N, st)) return rc;
+    if (d->dw) {
+      const Epilogue e = {nullptr, nullptr, d->dw, nullptr, 0, (long)d->K, HI3D_F32, HI3D_ACT_NONE};
+      const dim3 grid(grid_of((long)d->N * ((d->K + 7) / 8)));
+      if (d->dtype == HI3D_BF16) hipLaunchKernelGGL((join_kernel<bf16_t>), grid, dim3(256), 0, st, nullptr, e, (long)d->N, d->K, 0);
+      else hipLaunchKernelGGL((join_kernel<half_t>), grid, dim3(256), 0, st, nullptr, e, (long)d->N, d->K, 0);
+      HI3D_LAUNCH_CHECK();
+    }
+    return 0;
+  }
+  if (!d->dy || (d->dx && !d->w) || (d->dw && !d->x) || (d->act != HI3D_ACT_NONE && !d->z)) HI3D_FAIL(HI3D_EINVAL, "linear_bwd: null pointer");
+  if ((d->M > 1 && (d->lddy < d->N || (d->act != HI3D_ACT_NONE && d->ldz < d->N) || (d->dw && d->ldx < d->K))) || (d->dx && d->N > 1 && d->ldw < d->K))
+    HI3D_FAIL(HI3D_EINVAL, "linear_bwd: row pitch below the width");
+  const int64_t need = hi3d_linear_bwd_workspace_bytes(d);
+  if (need && (!d->ws || d->ws_bytes < need || ((uintptr_t)d->ws & 255))) HI3D_FAIL(HI3D_EINVAL, "linear_bwd: workspace missing, too small or not 256-byte aligned");
+  return d->dtype == HI3D_BF16 ? bwd<bf16_t>(d, st) : bwd<half_t>(d, st);
+}

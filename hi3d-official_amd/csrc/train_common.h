@@ -87,6 +87,13 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
+}  // namespace
+
+// o0[0, C) and o1[0, width - C) = the column sums of part[nblk][width], in a fixed order (norm_train.hip)
+int hi3d_column_reduce(const float* part, void* o0, void* o1, int code0, int code1, int nblk, int C, int width, hipStream_t st);
+
+namespace {
+
 inline bool hi3d_known_dtype(int c) { return c == HI3D_F32 || c == HI3D_BF16 || c == HI3D_F16; }
 inline int hi3d_dtype_size(int c) { return c == HI3D_F32 ? 4 : 2; }
 

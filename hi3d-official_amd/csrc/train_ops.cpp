@@ -133,6 +133,85 @@ std::tuple<Tensor, Tensor, Tensor> layernorm_bwd(const Tensor& dy, const Tensor&
   return {dx, dw, db};
 }
 
+// ---- linear layer -----------------------------------------------------------------------------------------------------------------
+int act_of(c10::string_view a, const char* name) {
+  if (a == "none") return HI3D_ACT_NONE;
+  if (a == "gelu") return HI3D_ACT_GELU;
+  if (a == "quick_gelu") return HI3D_ACT_QUICK_GELU;
+  if (a == "silu") return HI3D_ACT_SILU;
+  if (a == "relu") return HI3D_ACT_RELU;
+  TORCH_CHECK(false, name, ": unknown activation '", a, "' (none, gelu, quick_gelu, silu, relu)");
+}
+// sizes, types and activation of a call on x [M, K], w [N, K], bias [N]
+hi3d_linear_desc linear_desc(const Tensor& x, const Tensor& w, const OptTensor& bias, c10::string_view act, const char* name) {
+  want_gpu(x, x, name);
+  want_gpu(w, x, name);
+  TORCH_CHECK(x.dim() == 2 && w.dim() == 2 && x.size(1) == w.size(1) && x.size(1) >= 1 && w.size(0) >= 1, name, ": x [M, K] and w [N, K] of at least one column required");
+  TORCH_CHECK(x.scalar_type() == w.scalar_type() && (x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf), name, ": x and w must both be bf16 or both fp16");
+  TORCH_CHECK(w.size(0) <= 0x7fffffffLL && w.size(1) <= 0x7fffffffLL, name, ": a width does not fit 32 bits");
+  hi3d_linear_desc d = {};
+  d.M = x.size(0); d.N = (int32_t)w.size(0); d.K = (int32_t)w.size(1);
+  d.dtype = dtype_of(x, name); d.bias_dtype = HI3D_F32; d.act = act_of(act, name);
+  if (has(bias)) {
+    want_gpu(*bias, x, name);
+    TORCH_CHECK(bias->dim() == 1 && bias->size(0) == d.N && (bias->scalar_type() == at::kFloat || bias->scalar_type() == x.scalar_type()), name,
+                ": bias must be [N], fp32 or of x's type");
+    d.bias_dtype = dtype_of(*bias, name);
+  }
+  return d;
+}
+void want_like(const Tensor& t, const Tensor& x, int64_t M, int64_t N, const char* name, const char* what) {
+  want_gpu(t, x, name);
+  TORCH_CHECK(t.dim() == 2 && t.size(0) == M && t.size(1) == N && t.scalar_type() == x.scalar_type(), name, ": ", what, " must be [", M, ", ", N, "] of x's type");
+}
+Tensor workspace(hi3d_linear_desc* d, int64_t bytes, const Tensor& on) {
+  Tensor ws;
+  if (bytes) {
+    ws = at::empty({bytes}, on.options().dtype(at::kByte));
+    d->ws = ws.data_ptr(); d->ws_bytes = bytes;
+  }
+  return ws;
+}
+
+std::tuple<Tensor, Tensor> linear_act(const Tensor& x, const Tensor& w, const OptTensor& bias, const OptTensor& residual, c10::string_view act, bool save_z) {
+  const char* name = "hi3d::linear_act";
+  hi3d_linear_desc d = linear_desc(x, w, bias, act, name);
+  if (has(residual)) want_like(*residual, x, d.M, d.N, name, "residual");
+  const Guard guard(x.device());
+  const Rows rx = rows_of(x), rw = rows_of(w), rr = has(residual) ? rows_of(*residual) : Rows{Tensor(), 0, 0, 0};
+  const Tensor b = dense(bias);
+  Tensor y = at::empty({d.M, d.N}, x.options()), z;
+  if (save_z) z = at::empty({d.M, d.N}, x.options());
+  d.x = rx.t.data_ptr(); d.ldx = rx.ld; d.w = rw.t.data_ptr(); d.ldw = rw.ld;
+  d.bias = b.defined() ? b.data_ptr() : nullptr;
+  if (rr.t.defined()) { d.residual = rr.t.data_ptr(); d.ldr = rr.ld; }
+  d.y = y.data_ptr(); d.z = z.defined() ? z.data_ptr() : nullptr;
+  const Tensor ws = workspace(&d, hi3d_linear_fwd_workspace_bytes(&d), x);
+  check_rc(hi3d_linear_fwd(&d, stream_of(x)), "hi3d_linear_fwd");
+  return {y, z};
+}
+
+std::tuple<Tensor, Tensor, Tensor> linear_act_bwd(const Tensor& dy, const Tensor& x, const Tensor& w, const OptTensor& z, const OptTensor& bias, c10::string_view act,
+                                                  bool need_dx, bool need_dw) {
+  const char* name = "hi3d::linear_act_bwd";
+  hi3d_linear_desc d = linear_desc(x, w, bias, act, name);
+  want_like(dy, x, d.M, d.N, name, "dy");
+  TORCH_CHECK(d.act == HI3D_ACT_NONE || has(z), name, ": this activation's gradient needs z");
+  if (has(z)) want_like(*z, x, d.M, d.N, name, "z");
+  const Guard guard(x.device());
+  const Rows ry = rows_of(dy), rz = d.act != HI3D_ACT_NONE ? rows_of(*z) : Rows{Tensor(), 0, 0, 0}, rx = rows_of(x), rw = rows_of(w);
+  Tensor dx, dw, db;
+  if (need_dx) dx = at::empty({d.M, d.K}, x.options());
+  if (need_dw) dw = at::empty({d.N, d.K}, w.options());
+  if (has(bias)) db = at::empty({d.N}, bias->options());
+  d.x = rx.t.data_ptr(); d.ldx = rx.ld; d.w = rw.t.data_ptr(); d.ldw = rw.ld; d.dy = ry.t.data_ptr(); d.lddy = ry.ld;
+  if (rz.t.defined()) { d.z = rz.t.data_ptr(); d.ldz = rz.ld; }
+  d.dx = dx.defined() ? dx.data_ptr() : nullptr; d.dw = dw.defined() ? dw.data_ptr() : nullptr; d.db = db.defined() ? db.data_ptr() : nullptr;
+  const Tensor ws = workspace(&d, hi3d_linear_bwd_workspace_bytes(&d), x);
+  check_rc(hi3d_linear_bwd(&d, stream_of(x)), "hi3d_linear_bwd");
+  return {dx, dw, db};
+}
+
 // ---- AdamW ------------------------------------------------------------------------------------------------------------------------
 const float* scalar_of(const OptTensor& t, const Tensor& on, const char* what) {
   if (!has(t)) return nullptr;
@@ -207,8 +286,9 @@ void adamw_(at::TensorList params, at::TensorList grads, at::TensorList exp_avg,
   if (has(step_t)) {
     float* st = (float*)scalar_of(step_t, on, "hi3d::adamw_ step");
     coefs = at::empty({HI3D_ADAMW_COEFS}, on.options().dtype(at::kFloat).memory_format(c10::nullopt));
+    const hi3d_adamw_rates rates = {lr, beta1, beta2, weight_decay};
     check_rc(hi3d_adamw_coefs(coefs.data_ptr<float>(), st, scalar_of(lr_t, on, "hi3d::adamw_ lr"), scalar_of(grad_scale, on, "hi3d::adamw_ grad_scale"),
-                              scalar_of(found_inf, on, "hi3d::adamw_ found_inf"), lr, beta1, beta2, weight_decay, stream_of(on)), "hi3d_adamw_coefs");
+                              scalar_of(found_inf, on, "hi3d::adamw_ found_inf"), &rates, stream_of(on)), "hi3d_adamw_coefs");
   } else {
     c.shrink = (float)(1.0 - lr * weight_decay);
     c.step_size = (float)(lr / (1.0 - std::pow(beta1, (double)step)));
@@ -216,6 +296,10 @@ void adamw_(at::TensorList params, at::TensorList grads, at::TensorList exp_avg,
   }
   for (const Kind& k : kinds)
     check_rc(hi3d_adamw_step(k.t.data(), (int)k.t.size(), k.p, k.g, k.c, &c, coefs.defined() ? coefs.data_ptr<float>() : nullptr, stream_of(on)), "hi3d_adamw_step");
+  // a backward pass that saved these before the step has to see that they changed
+  for (const at::TensorList& l : {params, copies})
+    for (const Tensor& t : l)
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 }  // namespace
@@ -224,6 +308,8 @@ TORCH_LIBRARY_FRAGMENT(hi3d, m) {
   m.def("layernorm_fwd(Tensor x, Tensor? weight, Tensor? bias, float eps) -> (Tensor, Tensor, Tensor)");
   m.def("add_layernorm_fwd(Tensor x, Tensor residual, Tensor? weight, Tensor? bias, float eps) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("layernorm_bwd(Tensor dy, Tensor z, Tensor mean, Tensor rstd, Tensor? weight, Tensor? bias, Tensor? dz) -> (Tensor, Tensor, Tensor)");
+  m.def("linear_act(Tensor x, Tensor w, Tensor? bias, Tensor? residual, str act, bool save_z) -> (Tensor, Tensor)");
+  m.def("linear_act_bwd(Tensor dy, Tensor x, Tensor w, Tensor? z, Tensor? bias, str act, bool need_dx, bool need_dw) -> (Tensor, Tensor, Tensor)");
   m.def("adamw_(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avg, Tensor(c!)[] exp_avg_sq, Tensor(d!)[] copies, float lr, float beta1, "
         "float beta2, float eps, float weight_decay, int step, Tensor(e!)? step_t, Tensor? lr_t, Tensor? grad_scale, Tensor? found_inf) -> ()");
 }
@@ -232,5 +318,7 @@ TORCH_LIBRARY_IMPL(hi3d, CUDA, m) {
   m.impl("layernorm_fwd", &layernorm_fwd);
   m.impl("add_layernorm_fwd", &add_layernorm_fwd);
   m.impl("layernorm_bwd", &layernorm_bwd);
+  m.impl("linear_act", &linear_act);
+  m.impl("linear_act_bwd", &linear_act_bwd);
   m.impl("adamw_", &adamw_);
 }

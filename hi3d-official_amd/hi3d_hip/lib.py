@@ -23,6 +23,7 @@ EXPORTS = [
     "hi3d_act_bf16", "hi3d_l2_normalize_rows", "hi3d_add_act_bf16", "hi3d_dpt_stem_conv", "hi3d_pool2_nhwc",
     "hi3d_resize_bilinear_nhwc", "hi3d_dpt_head_out", "hi3d_depth_normalize_unshuffle", "hi3d_resample_axis", "hi3d_permute_rows",
     "hi3d_layernorm_fwd", "hi3d_layernorm_bwd_workspace_floats", "hi3d_layernorm_bwd", "hi3d_adamw_coefs", "hi3d_adamw_step",
+    "hi3d_linear_fwd_workspace_bytes", "hi3d_linear_fwd", "hi3d_linear_bwd_workspace_bytes", "hi3d_linear_bwd",
 ]
 
 ABI_VERSION = 3          # == HI3D_ABI_VERSION of the include/hi3d_hip.h this binding was written against (GemmDesc below is that layout)
@@ -127,7 +128,11 @@ def load():
         "hi3d_layernorm_fwd": (C.c_int, [vp] * 8 + [i64, i32, i64, i64, i32, i32, f32, vp]),
         "hi3d_layernorm_bwd_workspace_floats": (i64, [i64, i32, i32]),
         "hi3d_layernorm_bwd": (C.c_int, [vp] * 10 + [i64, i32, i64, i64, i64, i32, i32, vp]),
-        "hi3d_adamw_coefs": (C.c_int, [vp] * 5 + [C.c_double] * 4 + [vp]),
+        "hi3d_linear_fwd_workspace_bytes": (i64, [vp]),
+        "hi3d_linear_fwd": (C.c_int, [vp, vp]),
+        "hi3d_linear_bwd_workspace_bytes": (i64, [vp]),
+        "hi3d_linear_bwd": (C.c_int, [vp, vp]),
+        "hi3d_adamw_coefs": (C.c_int, [vp] * 7),
         "hi3d_adamw_step": (C.c_int, [vp, i32, i32, i32, i32, vp, vp, vp]),
     }
     for name, (res, args) in sig.items():

@@ -20,7 +20,7 @@ from . import lib as _l
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libhi3d_torch.so")
 OPS = ("self_attention", "attn_d64", "attn_temporal", "groupnorm_silu", "layernorm", "linear", "conv3x3", "ffn_geglu",
-       "layernorm_fwd", "add_layernorm_fwd", "layernorm_bwd", "adamw_")
+       "layernorm_fwd", "add_layernorm_fwd", "layernorm_bwd", "linear_act", "linear_act_bwd", "adamw_")
 _loaded = False
 
 

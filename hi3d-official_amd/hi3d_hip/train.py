@@ -6,10 +6,12 @@ trained through the operator binding:
     from hi3d_hip import train
     y = train.layer_norm(x, weight, bias)                       # nn.LayerNorm
     y, z = train.layer_norm(x, weight, bias, residual=r)        # z = x + r, y = LayerNorm(z)
+    y = train.linear(x, w, bias, residual=r, act="gelu")        # act(x w^T + bias) + r
     opt = train.AdamW(model.parameters(), lr=1e-5)              # torch.optim.AdamW
 
 `AdamW` is a torch.optim.Optimizer and so a `target:` of the reference's YAML (`optimizer_config`).  Underneath are
-torch.ops.hi3d.layernorm_fwd / add_layernorm_fwd / layernorm_bwd / adamw_, which may be called by themselves: a step that is
+torch.ops.hi3d.layernorm_fwd / add_layernorm_fwd / layernorm_bwd / linear_act /
+linear_act_bwd / adamw_, which may be called by themselves: a step that is
 captured into a HIP graph calls these, since a captured autograd backward shares its leaves' gradient nodes -- and the
 stream they were made on -- with any eager graph of the same leaves that is still alive.
 """
@@ -49,12 +51,43 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
     return _LayerNorm.apply(x, residual, weight, bias, float(eps))
 
 
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, residual, act):
+        y, z = torch_ops.load().linear_act(x, w, bias, residual, act, act != "none" and any(ctx.needs_input_grad[:3]))
+        ctx.act = act
+        ctx.save_for_backward(x, w, bias, z)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w, bias, z = ctx.saved_tensors
+        nx, nw, nb, nr, _ = ctx.needs_input_grad
+        dx = dw = db = None
+        if nx or nw or nb:
+            dx, dw, db = torch_ops.load().linear_act_bwd(dy, x, w, z, bias if nb else None, ctx.act, nx, nw)
+        return dx, dw, db, dy if nr else None, None
+
+
+def linear(x, w, bias=None, residual=None, act="none"):
+    """act(x w^T + bias) (+ residual), differentiable.  x [..., K], w [N, K] (nn.Linear's): bf16 or fp16, any sizes and strides; bias [N]:
+    fp32 or x's type; residual [..., N] of x's type and exactly the result's shape; act: "none", "gelu" (exact), "quick_gelu", "silu",
+    "relu".  Products and sums are fp32; the gradients' products take dy act'(z) rounded to x's type, z being kept in it."""
+    lead = x.shape[:-1]
+    if residual is not None:
+        if residual.shape != (*lead, w.shape[0]):
+            raise _l.Hi3dError(f"linear: residual must be {tuple(lead) + (w.shape[0],)}, got {tuple(residual.shape)}")
+        residual = residual.reshape(-1, w.shape[0])
+    return _Linear.apply(x.reshape(-1, x.shape[-1]), w, bias, residual, act).reshape(*lead, w.shape[0])
+
+
 class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's update for all tensors of a group in one launch per 72 of them (torch.ops.hi3d.adamw_).
 
     Parameters fp32, bf16 or fp16 on one GPU, dense in memory; moments are fp32 whatever the parameter's type.
     working_dtype (torch.bfloat16 / torch.float16): fp32 parameters keep a copy in that type which every step rewrites -- the
-    weights the forward pass reads, `working_copy(p)`.
+    weights that the forward pass reads, `working_copy(p)`, a leaf with a gradient of its own: step() takes that one where p has none.
     capturable: step count on the device (per group: each of its parameters then needs a gradient at every step), so that step() can be
     captured into a HIP graph; `lr` may then be a one-element fp32 device tensor.  torch.amp.GradScaler's scale and
     overflow flag are read on the device in this mode.
@@ -77,7 +110,7 @@ class AdamW(torch.optim.Optimizer):
         self._step_supports_amp_scaling = all(g["capturable"] for g in self.param_groups)
 
     def working_copy(self, p):
-        """The 16-bit copy of parameter p that step() keeps (its value before the first step: p rounded)."""
+        """The 16-bit copy of parameter p that step() keeps (before the first step: p rounded)."""
         return self._state_of(p, self._group_of(p))["copy"]
 
     def _group_of(self, p):
@@ -97,8 +130,23 @@ class AdamW(torch.optim.Optimizer):
             if group["working_dtype"] is not None:
                 if p.dtype != torch.float32:
                     raise _l.Hi3dError("a working copy is kept of fp32 parameters only")
-                s["copy"] = p.detach().to(group["working_dtype"])
+                s["copy"] = p.detach().to(group["working_dtype"]).requires_grad_(p.requires_grad)
         return s
+
+    def _grad(self, p):
+        if p.grad is not None or "copy" not in self.state.get(p, ()):
+            return p.grad
+        return self.state[p]["copy"].grad
+
+    def zero_grad(self, set_to_none=True):
+        super().zero_grad(set_to_none)
+        for s in self.state.values():
+            c = s.get("copy")
+            if c is not None and c.grad is not None:
+                if set_to_none:
+                    c.grad = None
+                else:
+                    c.grad.zero_()
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -109,12 +157,12 @@ class AdamW(torch.optim.Optimizer):
         ns = torch_ops.load()
         scale, found_inf = getattr(self, "grad_scale", None), getattr(self, "found_inf", None)
         for group in self.param_groups:
-            with_grad = [p for p in group["params"] if p.grad is not None]
+            with_grad = [p for p in group["params"] if self._grad(p) is not None]
             if group["capturable"] and with_grad and len(with_grad) < len(group["params"]):
                 raise _l.Hi3dError("capturable: every parameter of the group needs a gradient at every step")
             by_step = {}                                    # (one list, unless some parameters had no gradient at earlier steps)
             for p in with_grad:
-                g = p.grad
+                g = self._grad(p)
                 if g.is_sparse:
                     raise _l.Hi3dError("sparse gradients are not supported")
                 if g.stride() != p.stride():
@@ -138,13 +186,18 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        """As torch's, but the moments and copies keep their own types (torch casts a state to its parameter's type)."""
+        """As torch's, but the moments and copies keep their own types (torch casts a state to its parameter's type), and working
+        copies that have been handed out take the loaded values."""
+        copies = {p: s["copy"] for p, s in self.state.items() if "copy" in s}
         super().load_state_dict(state_dict)
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
             for k, v in state_dict["state"].get(i, {}).items():
                 if torch.is_tensor(v):
-                    self.state[p][k] = torch.empty_like(p, dtype=v.dtype).copy_(v)
+                    with torch.no_grad():
+                        to = copies[p] if k == "copy" and p in copies and copies[p].dtype == v.dtype else torch.empty_like(p, dtype=v.dtype, requires_grad=False)
+                        to.copy_(v)
+                    self.state[p][k] = to.requires_grad_(p.requires_grad) if k == "copy" else to
         for g in self.param_groups:
             if g["step_t"] is not None and g["params"]:
                 g["step_t"] = g["step_t"].detach().clone().to(g["params"][0].device)

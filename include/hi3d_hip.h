@@ -342,6 +342,35 @@ int hi3d_layernorm_bwd(const void* dy, const void* z, const void* dz, const void
                        const float* rstd, void* dx, void* dweight, void* dbias, float* ws, int64_t R, int32_t C,
                        int64_t lddy, int64_t ldz, int64_t lddz, int32_t dtype, int32_t wdtype, void* stream);
 
+/* A linear layer with its epilogue, and its gradients (beside hi3d_gemm_bf16: any sizes, pitches and alignments, an activation in the
+ * epilogue, bf16 or fp16):
+ *   fwd: z = x w^T + bias;  y = act(z) (+ residual)            x [M][K] pitch ldx, w [N][K] pitch ldw, residual [M][N] pitch ldr
+ *        y, z (NULL: not kept): dense [M][N], `dtype`, each one rounding of the fp32 result
+ *   bwd: dz = dy act'(z);  dx = dz w;  dw = dz^T x;  db = sum_m dz    dy [M][N] pitch lddy, z [M][N] pitch ldz (not read for
+ *        HI3D_ACT_NONE), dx dense [M][K], dw dense [N][K] (`dtype`), db [N] (`bias_dtype`); each of dx, dw, db may be NULL.
+ *        dz is rounded to `dtype` for the products (their sums are fp32); db sums it unrounded.  Fixed order of all sums.
+ * bias, db: `bias_dtype`, HI3D_F32 or `dtype`.  act: HI3D_ACT_*; GELU is the exact one, QUICK_GELU z * sigmoid(1.702 z).
+ * ws: ..._workspace_bytes(d) bytes, 256-byte aligned (that function reads all fields but ws).  Outputs overlap nothing.  M = 0: db and dw are zeros, nothing else is written. */
+#define HI3D_ACT_NONE 0
+#define HI3D_ACT_GELU 1
+#define HI3D_ACT_QUICK_GELU 2
+#define HI3D_ACT_SILU 3
+#define HI3D_ACT_RELU 4
+typedef struct {
+  const void *x, *w, *bias, *residual;
+  void *y, *z;
+  const void* dy;
+  void *dx, *dw, *db;
+  int64_t M, ldx, ldw, ldr, lddy, ldz;
+  int32_t N, K, dtype, bias_dtype, act;
+  void* ws;
+  int64_t ws_bytes;
+} hi3d_linear_desc;
+int64_t hi3d_linear_fwd_workspace_bytes(const hi3d_linear_desc* d);
+int hi3d_linear_fwd(const hi3d_linear_desc* d, void* stream);
+int64_t hi3d_linear_bwd_workspace_bytes(const hi3d_linear_desc* d);
+int hi3d_linear_bwd(const hi3d_linear_desc* d, void* stream);
+
 /* One AdamW step over n tensors (decoupled weight decay; 32-bit moments), in place:
  *   m <- beta1 m + (1 - beta1) g';  v <- beta2 v + (1 - beta2) g'^2;  p <- p * shrink - step_size * m / (sqrt(v) * inv_root + eps)
  * with g' = g * grad_scale, shrink = 1 - lr * weight_decay, step_size = lr / (1 - beta1^t), inv_root = 1 / sqrt(1 - beta2^t).
@@ -351,13 +380,14 @@ int hi3d_layernorm_bwd(const void* dy, const void* z, const void* dz, const void
  *
  * hi3d_adamw_coefs: the four (and a flag) for a step whose count lives on the device: *step += 1, unless *found_inf (may be NULL) is
  * not zero -- then the count stays and hi3d_adamw_step with this output changes nothing.  out: HI3D_ADAMW_COEFS floats.  lr_dev
- * replaces lr; grad_scale is the loss scale, by which gradients are divided (either may be NULL).       */
+ * replaces rates->lr; grad_scale is the loss scale, by which gradients are divided (either may be NULL).       */
 typedef struct { void* p; const void* g; float* m; float* v; void* copy; int64_t n; } hi3d_adamw_tensor;
 typedef struct { float shrink, step_size, inv_root, grad_scale, beta1, one_minus_beta1, beta2, one_minus_beta2, eps; } hi3d_adamw_coefs_t;
+typedef struct { double lr, beta1, beta2, weight_decay; } hi3d_adamw_rates;
 #define HI3D_ADAMW_SKIP 4
 #define HI3D_ADAMW_COEFS 8
 int hi3d_adamw_coefs(float* out, float* step, const float* lr_dev, const float* grad_scale, const float* found_inf,
-                     double lr, double beta1, double beta2, double weight_decay, void* stream);
+                     const hi3d_adamw_rates* rates, void* stream);
 int hi3d_adamw_step(const hi3d_adamw_tensor* t, int32_t n, int32_t pdtype, int32_t gdtype, int32_t copy_dtype,
                     const hi3d_adamw_coefs_t* c, const float* coefs_dev, void* stream);
 

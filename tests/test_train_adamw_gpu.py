@@ -215,6 +215,13 @@ def test_optimiser_is_torchs(dev):
     o.step()
     o2 = train.AdamW([b])
     o2.load_state_dict(o.state_dict())
+    w = torch.nn.Parameter(torch.randn(10, device=dev))
+    o3, o4 = train.AdamW([w], working_dtype=torch.bfloat16), train.AdamW([w], working_dtype=torch.bfloat16)
+    held = o4.working_copy(w)
+    o3.working_copy(w).grad = torch.ones(10, device=dev).bfloat16()
+    o3.step()
+    o4.load_state_dict(o3.state_dict())
+    assert o4.working_copy(w) is held and torch.equal(held, w.bfloat16()) and held.requires_grad and held.is_leaf
     assert o2.state[b]["exp_avg"].dtype == torch.float32 and torch.equal(o2.state[b]["exp_avg"], o.state[b]["exp_avg"]) and o2.state[b]["step"] == 1
 
 

@@ -52,7 +52,45 @@ def test_adamw_refuses(lib):
     for t, n, kw in ((None, 1, {}), (ok, -1, {}), (ok, 1, dict(pd=BAD_TYPE)), (ok, 1, dict(gd=BAD_TYPE)), (ok, 1, dict(cd=F32)), (ok, 1, dict(c=None)),
                      (T(0, P, P, P, 0, 4), 1, {}), (T(P, 0, P, P, 0, 4), 1, {}), (T(P, P, 0, P, 0, 4), 1, {}), (T(P, P, P, 0, 0, 4), 1, {}), (T(P, P, P, P, 0, -4), 1, {})):
         assert step(t, n, **kw) < 0
-    assert lib.hi3d_adamw_coefs(0, P, 0, 0, 0, 1.0, 0.9, 0.99, 0.0, 0) < 0 and lib.hi3d_adamw_coefs(P, 0, 0, 0, 0, 1.0, 0.9, 0.99, 0.0, 0) < 0
+    for k in (0, 1, 5):
+        assert lib.hi3d_adamw_coefs(*[0 if i == k else P if i in (0, 1, 5) else 0 for i in range(6)], 0) < 0
+
+
+class Linear(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("x", "w", "bias", "residual", "y", "z", "dy", "dx", "dw", "db")] + \
+               [(n, C.c_int64) for n in ("M", "ldx", "ldw", "ldr", "lddy", "ldz")] + [(n, C.c_int32) for n in ("N", "K", "dtype", "bias_dtype", "act")] + \
+               [("ws", C.c_void_p), ("ws_bytes", C.c_int64)]
+
+
+def linear(**k):
+    a = dict(x=P, w=P, bias=P, residual=0, y=P, z=0, dy=P, dx=P, dw=P, db=P, M=64, ldx=64, ldw=64, ldr=64, lddy=64, ldz=64, N=64, K=64, dtype=BF16, bias_dtype=F32, act=0,
+             ws=P, ws_bytes=1 << 40) | k
+    return Linear(**{n: (a[n] or None) if t is C.c_void_p else a[n] for n, t in Linear._fields_})
+
+
+@pytest.mark.parametrize("k", [dict(x=0), dict(w=0), dict(M=-1), dict(N=0), dict(K=0), dict(dtype=F32), dict(dtype=BAD_TYPE), dict(bias_dtype=2), dict(act=5), dict(act=-1),
+                               dict(ldw=63), dict(ldx=63), dict(K=63, ldx=63, ws=0), dict(K=63, ws_bytes=10), dict(K=63, ws=P + 8), dict(K=1 << 22, ldx=1 << 22, ldw=1 << 22),
+                               dict(N=1 << 22), dict(ldx=1 << 30), dict(M=1 << 31)])
+def test_linear_refuses(lib, k):
+    d = linear(**k)
+    assert lib.hi3d_linear_fwd(C.addressof(d), 0) < 0 and lib.hi3d_last_error()
+
+
+@pytest.mark.parametrize("k", [dict(dy=0), dict(x=0), dict(w=0), dict(act=1), dict(act=1, z=P, ldz=63), dict(lddy=63), dict(ldx=63), dict(ldw=63), dict(db=P, ws=0), dict(M=1 << 31),
+                               dict(act=1, z=P, ws_bytes=64 * 64 * 2)])
+def test_linear_bwd_refuses(lib, k):
+    d = linear(**k)
+    assert lib.hi3d_linear_bwd(C.addressof(d), 0) < 0 and lib.hi3d_last_error()
+
+
+def test_linear_null_and_empty(lib):
+    assert lib.hi3d_linear_fwd(0, 0) < 0 and lib.hi3d_linear_bwd(0, 0) < 0
+    assert lib.hi3d_linear_fwd_workspace_bytes(0) == 0 and lib.hi3d_linear_bwd_workspace_bytes(0) == 0
+    assert lib.hi3d_linear_fwd(C.addressof(linear(M=0, x=0, y=0)), 0) == 0
+    assert lib.hi3d_linear_bwd(C.addressof(linear(M=0, dy=0, dw=0, db=0)), 0) == 0
+    # rows of 63 elements cannot be read in place: both operands are copied; 64 can
+    assert lib.hi3d_linear_fwd_workspace_bytes(C.addressof(linear(M=1024, N=1024, K=64))) == 0
+    assert lib.hi3d_linear_fwd_workspace_bytes(C.addressof(linear(M=1024, N=1024, K=63))) == 2 * 1024 * 64 * 2
 
 
 def test_cpu_tensors_are_refused():
@@ -60,6 +98,7 @@ def test_cpu_tensors_are_refused():
     ns = torch_ops.load()
     x = torch.zeros(2, 4)
     for f in (lambda: ns.layernorm_fwd(x, None, None, 1e-5), lambda: ns.add_layernorm_fwd(x, x, None, None, 1e-5), lambda: train.layer_norm(x),
+              lambda: ns.linear_act(x, x, None, None, "none", False), lambda: ns.linear_act_bwd(x[:, :2], x, x, None, None, "none", True, True),
               lambda: ns.adamw_([x], [x], [x], [x], [], 0.1, 0.9, 0.99, 1e-8, 0.0, 1, None, None, None, None)):
         with pytest.raises((RuntimeError, NotImplementedError)):
             f()
