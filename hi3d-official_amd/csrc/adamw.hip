@@ -59,10 +59,10 @@ __global__ __launch_bounds__(THR) void adamw_kernel(const AdamwArgs a) {
       e[u] = base + ((h * UNROLL + u) * THR + threadIdx.x) * V;
       const long left = count - e[u];
       n[u] = left < V ? (int)(left < 0 ? 0 : left) : V;
-      fetch(p + e[u], n[u], kp[u]);
-      fetch(g + e[u], n[u], kg[u]);
-      fetch(m + e[u], n[u], km[u]);
-      fetch(v + e[u], n[u], kv[u]);
+      fetch(p + e[u], n[u], e[u], kp[u]);
+      fetch(g + e[u], n[u], e[u], kg[u]);
+      fetch(m + e[u], n[u], e[u], km[u]);
+      fetch(v + e[u], n[u], e[u], kv[u]);
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {

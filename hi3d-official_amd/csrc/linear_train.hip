@@ -8,7 +8,6 @@
 // contraction (KC: x and w forward, dz for dx) or across it (KS: w for dx, both for dw), and a KS tile reaches the matrix instruction
 // through gfx950's transposing LDS read, so nothing is transposed in memory.
 #include "train_common.h"
-#include <type_traits>
 
 namespace {
 
@@ -89,7 +88,7 @@ __device__ __forceinline__ void finish(const Epilogue& e, long m, int c, int n, 
   if (e.res) {
     Pack<T, 8> k;
     float r[8];
-    fetch((const T*)e.res + m * e.ldr + c, n, k);
+    fetch((const T*)e.res + m * e.ldr + c, n, c, k);
     unpack(k, r);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] += r[j];
@@ -341,9 +340,9 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, Epilogue e
     float v[8] = {};
     for (int s = 0; s < splits; ++s) {
       Pack<float, 8> k;
-      fetch(part + (s * M + m) * N + n, N - n, k);
+      fetch(part + (s * M + m) * N + n, N - n, n, k);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += k.v[j];
+      for (int j = 0; j < 8; ++j) v[j] += __uint_as_float(k.w[j]);
     }
     finish<T>(e, m, n, N - n, v);
   }
@@ -357,7 +356,7 @@ __global__ __launch_bounds__(256) void pad_kernel(const T* in, T* out, long rows
     const long r = c / cpr;
     const int e = (int)(c - r * cpr) * 8;
     Pack<T, 8> k;
-    fetch(in + r * ld + e, cols - e, k);
+    fetch(in + r * ld + e, cols - e, e, k);
     *(Pack<T, 8>*)(out + r * (long)cpr * 8 + e) = k;
   }
 }
@@ -380,8 +379,8 @@ __global__ __launch_bounds__(256) void slope_kernel(const SlopeParams p) {
     for (long r = r0 + ty; r < r1; r += 8) {
       Pack<T, 8> ky, kz;
       float v[8], z[8];
-      fetch((const T*)p.dy + r * p.lddy + c, n, ky);
-      if (p.act) fetch((const T*)p.z + r * p.ldz + c, n, kz);
+      fetch((const T*)p.dy + r * p.lddy + c, n, c, ky);
+      if (p.act) fetch((const T*)p.z + r * p.ldz + c, n, c, kz);
       unpack(ky, v);
       if (p.act) {
         unpack(kz, z);

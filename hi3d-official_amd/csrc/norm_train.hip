@@ -32,6 +32,60 @@ struct NormBwdParams {
 
 constexpr int NTHR = 256;
 
+// A row's vectors as one lane holds them: vector i covers elements at[i] ... at[i] + V of the row, n[i] of which exist.  The one that the
+// row's end cuts is read so that it ends there and moved down once all of the row's loads are out (`settle`).  TINY: rows shorter than a
+// vector, element by element.
+template <typename T, int LPR, int NV, bool TINY>
+struct RowMap {
+  static constexpr int V = Elem<T>::VEC;
+  int n[NV];
+  bool ragged;
+  __device__ __forceinline__ RowMap(int l, int C) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) n[i] = C - (l + i * LPR) * V;
+    ragged = C % V != 0;
+  }
+  __device__ __forceinline__ void load(const T* row, int l, bool in, Pack<T, V> (&k)[NV]) const {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = (l + i * LPR) * V;
+      if constexpr (TINY) fetch(row + e, in ? n[i] : 0, 0, k[i]);
+      else {
+#pragma unroll
+        for (int j = 0; j < Pack<T, V>::W; ++j) k[i].w[j] = 0;
+        if (in && n[i] > 0) k[i] = *(const Pack<T, V>*)(row + e - max(0, V - n[i]));
+      }
+    }
+  }
+  __device__ __forceinline__ void settle(Pack<T, V> (&k)[NV]) const {
+    if constexpr (!TINY)
+      if (ragged) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) shift_down(k[i], n[i] > 0 && n[i] < V ? V - n[i] : 0);
+      }
+  }
+  // a weight or bias of the run-time type `code` in the lane's columns (1 or 0 where there is none)
+  __device__ __forceinline__ void columns(const void* p, int code, int l, float none, float (&f)[NV][V]) const {
+    if (!p) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[i][j] = none;
+    } else if (code == HI3D_F32) columns_of((const float*)p, l, f);
+    else if (code == HI3D_BF16) columns_of((const bf16_t*)p, l, f);
+    else columns_of((const half_t*)p, l, f);
+  }
+  template <typename W>
+  __device__ __forceinline__ void columns_of(const W* p, int l, float (&f)[NV][V]) const {
+    Pack<W, V> k[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) fetch(p + (l + i * LPR) * V, n[i], (l + i * LPR) * V, k[i]);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) unpack(k[i], f[i]);
+  }
+  __device__ __forceinline__ void store(T* row, int l, bool in, int i, const float (&f)[V]) const { store_some(row + (l + i * LPR) * V, in ? n[i] : 0, f); }
+};
+
 // sum over the lanes that hold a row; the block form goes through LDS (`slot` alternates, so that one barrier per sum is enough)
 template <int LPR>
 __device__ __forceinline__ float row_sum(float v, float* lds, int& slot) {
@@ -44,23 +98,16 @@ __device__ __forceinline__ float row_sum(float v, float* lds, int& slot) {
   return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
-template <typename T, int LPR, int NV, bool ADD>
+template <typename T, int LPR, int NV, bool ADD, bool TINY>
 __global__ __launch_bounds__(NTHR) void norm_fwd_kernel(const NormFwdParams p) {
   constexpr int V = Elem<T>::VEC, RPB = NTHR / LPR;
   __shared__ float lds[8];
   int slot = 0;
   const int l = threadIdx.x % LPR, sub = threadIdx.x / LPR, C = p.C;
-  int n[NV];                                    // elements of this lane's i-th vector that exist
+  const RowMap<T, LPR, NV, TINY> map(l, C);
   float w[NV][V], b[NV][V];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int e = (l + i * LPR) * V;
-    n[i] = C - e;
-#pragma unroll
-    for (int j = 0; j < V; ++j) { w[i][j] = 1.0f; b[i][j] = 0.0f; }
-    if (p.w) load_vec_as(p.w, p.wcode, e, n[i], w[i]);
-    if (p.b) load_vec_as(p.b, p.wcode, e, n[i], b[i]);
-  }
+  map.columns(p.w, p.wcode, l, 1.0f, w);
+  map.columns(p.b, p.wcode, l, 0.0f, b);
   const bool ragged = C != LPR * NV * V;
   const float inv = 1.0f / (float)C;
   for (long r0 = (long)blockIdx.x * RPB; r0 < p.R; r0 += (long)gridDim.x * RPB) {
@@ -69,11 +116,9 @@ __global__ __launch_bounds__(NTHR) void norm_fwd_kernel(const NormFwdParams p) {
     float x[NV][V];
     float s = 0.0f;
     Pack<T, V> kx[NV], kr[ADD ? NV : 1];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      fetch((const T*)p.x + r * p.ldx + (l + i * LPR) * V, in ? n[i] : 0, kx[i]);
-      if constexpr (ADD) fetch((const T*)p.r + r * p.ldr + (l + i * LPR) * V, in ? n[i] : 0, kr[i]);
-    }
+    map.load((const T*)p.x + r * p.ldx, l, in, kx);
+    if constexpr (ADD) { map.load((const T*)p.r + r * p.ldr, l, in, kr); map.settle(kr); }
+    map.settle(kx);
 #pragma unroll
     for (int i = 0; i < NV; ++i) unpack(kx[i], x[i]);
     if constexpr (ADD) {
@@ -83,7 +128,7 @@ __global__ __launch_bounds__(NTHR) void norm_fwd_kernel(const NormFwdParams p) {
         unpack(kr[i], q[i]);
 #pragma unroll
         for (int j = 0; j < V; ++j) x[i][j] = Elem<T>::get(Elem<T>::put(x[i][j] + q[i][j]));   // the values the backward pass reads
-        store_some((T*)p.z + r * C + (l + i * LPR) * V, in ? n[i] : 0, x[i]);
+        map.store((T*)p.z + r * C, l, in, i, x[i]);
       }
     }
 #pragma unroll
@@ -95,7 +140,7 @@ __global__ __launch_bounds__(NTHR) void norm_fwd_kernel(const NormFwdParams p) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int j = 0; j < V; ++j) x[i][j] = j < n[i] ? x[i][j] : mu;
+        for (int j = 0; j < V; ++j) x[i][j] = j < map.n[i] ? x[i][j] : mu;
     }
     float q = 0.0f;
 #pragma unroll
@@ -108,7 +153,7 @@ __global__ __launch_bounds__(NTHR) void norm_fwd_kernel(const NormFwdParams p) {
       float y[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) y[j] = x[i][j] * rs * w[i][j] + b[i][j];
-      store_some((T*)p.y + r * C + (l + i * LPR) * V, in ? n[i] : 0, y);
+      map.store((T*)p.y + r * C, l, in, i, y);
     }
     if (in && l == 0) { p.mean[r] = mu; p.rstd[r] = rs; }
   }
@@ -116,36 +161,29 @@ __global__ __launch_bounds__(NTHR) void norm_fwd_kernel(const NormFwdParams p) {
 
 // the gradients of a block's rows: dx, and -- where they are asked for -- the block's sums of dy h and dy, in columns held by
 // the lane through all of its rows: nothing is added atomically, the order of the sums is that of the rows
-template <typename T, int LPR, int NV>
+template <typename T, int LPR, int NV, bool TINY>
 __global__ __launch_bounds__(NTHR) void norm_bwd_kernel(const NormBwdParams p) {
   constexpr int V = Elem<T>::VEC, RPB = NTHR / LPR;
   __shared__ float lds[8];
   __shared__ float cols[LPR <= 64 ? 4 * LPR * V : 1];
   int slot = 0;
   const int l = threadIdx.x % LPR, sub = threadIdx.x / LPR, C = p.C;
-  int n[NV];
-  float w[NV][V], gw[NV][V], gb[NV][V];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int e = (l + i * LPR) * V;
-    n[i] = C - e;
-#pragma unroll
-    for (int j = 0; j < V; ++j) { w[i][j] = 1.0f; gw[i][j] = gb[i][j] = 0.0f; }
-    if (p.w) load_vec_as(p.w, p.wcode, e, n[i], w[i]);
-  }
+  const RowMap<T, LPR, NV, TINY> map(l, C);
+  float w[NV][V], gw[NV][V] = {}, gb[NV][V] = {};
+  map.columns(p.w, p.wcode, l, 1.0f, w);
   const float inv = 1.0f / (float)C;
   for (long r0 = (long)blockIdx.x * RPB; r0 < p.R; r0 += (long)gridDim.x * RPB) {
     const long r = r0 + sub;
     const bool in = r < p.R;
     Pack<T, V> ky[NV], kz[NV], kd[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      fetch((const T*)p.dy + r * p.lddy + (l + i * LPR) * V, in ? n[i] : 0, ky[i]);     // (zero behind the row: adds nothing below)
-      fetch((const T*)p.z + r * p.ldz + (l + i * LPR) * V, in ? n[i] : 0, kz[i]);
-      if (p.dz) fetch((const T*)p.dz + r * p.lddz + (l + i * LPR) * V, in ? n[i] : 0, kd[i]);
-    }
+    map.load((const T*)p.dy + r * p.lddy, l, in, ky);                   // (zero behind the row: adds nothing below)
+    map.load((const T*)p.z + r * p.ldz, l, in, kz);
+    if (p.dz) map.load((const T*)p.dz + r * p.lddz, l, in, kd);
     const float mu = in ? p.mean[r] : 0.0f, rs = in ? p.rstd[r] : 0.0f;
     float dy[NV][V], h[NV][V];
+    map.settle(ky);
+    map.settle(kz);
+    if (p.dz) map.settle(kd);
 #pragma unroll
     for (int i = 0; i < NV; ++i) { unpack(ky[i], dy[i]); unpack(kz[i], h[i]); }
     float s1 = 0.0f, s2 = 0.0f;
@@ -153,7 +191,7 @@ __global__ __launch_bounds__(NTHR) void norm_bwd_kernel(const NormBwdParams p) {
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        h[i][j] = j < n[i] ? (h[i][j] - mu) * rs : 0.0f;
+        h[i][j] = j < map.n[i] ? (h[i][j] - mu) * rs : 0.0f;
         gb[i][j] += dy[i][j];
         gw[i][j] += dy[i][j] * h[i][j];
         dy[i][j] *= w[i][j];
@@ -173,7 +211,7 @@ __global__ __launch_bounds__(NTHR) void norm_bwd_kernel(const NormBwdParams p) {
 #pragma unroll
         for (int j = 0; j < V; ++j) o[j] += t[j];
       }
-      store_some((T*)p.dx + r * C + (l + i * LPR) * V, in ? n[i] : 0, o);
+      map.store((T*)p.dx + r * C, l, in, i, o);
     }
   }
   if (!p.want) return;
@@ -212,7 +250,7 @@ __global__ __launch_bounds__(NTHR) void norm_bwd_kernel(const NormBwdParams p) {
         const int e = (l + i * LPR) * V;
 #pragma unroll
         for (int j = 0; j < V; ++j)
-          if (j < n[i]) {
+          if (j < map.n[i]) {
             if (p.part) part[k * C + e + j] = t[j];
             else if (k ? p.db : p.dw) store_as(k ? p.db : p.dw, p.wcode, e + j, t[j]);
           }
@@ -251,11 +289,12 @@ Shape pick(int chunks) {
 }
 
 #define HI3D_NORM_SHAPES(LAUNCH)                                                                                  \
-  if (s.lpr == 8) { if (s.nv == 2) LAUNCH(8, 2); else if (s.nv == 3) LAUNCH(8, 3); else LAUNCH(8, 5); }           \
-  else if (s.lpr == 16) { if (s.nv == 3) LAUNCH(16, 3); else if (s.nv == 2) LAUNCH(16, 2); else LAUNCH(16, 5); }  \
-  else if (s.lpr == 32) { if (s.nv == 3) LAUNCH(32, 3); else if (s.nv == 2) LAUNCH(32, 2); else LAUNCH(32, 5); }  \
-  else if (s.lpr == 64) { if (s.nv == 3) LAUNCH(64, 3); else if (s.nv == 2) LAUNCH(64, 2); else LAUNCH(64, 5); }  \
-  else { if (s.nv == 2) LAUNCH(256, 2); else if (s.nv == 4) LAUNCH(256, 4); else LAUNCH(256, (Elem<T>::VEC == 8 ? 4 : 8)); }   /* 8192 wide */
+  if (p.C < Elem<T>::VEC) LAUNCH(8, 2, true); else                                                                                  \
+  if (s.lpr == 8) { if (s.nv == 2) LAUNCH(8, 2, false); else if (s.nv == 3) LAUNCH(8, 3, false); else LAUNCH(8, 5, false); }           \
+  else if (s.lpr == 16) { if (s.nv == 3) LAUNCH(16, 3, false); else if (s.nv == 2) LAUNCH(16, 2, false); else LAUNCH(16, 5, false); }  \
+  else if (s.lpr == 32) { if (s.nv == 3) LAUNCH(32, 3, false); else if (s.nv == 2) LAUNCH(32, 2, false); else LAUNCH(32, 5, false); }  \
+  else if (s.lpr == 64) { if (s.nv == 3) LAUNCH(64, 3, false); else if (s.nv == 2) LAUNCH(64, 2, false); else LAUNCH(64, 5, false); }  \
+  else { if (s.nv == 2) LAUNCH(256, 2, false); else if (s.nv == 4) LAUNCH(256, 4, false); else LAUNCH(256, (Elem<T>::VEC == 8 ? 4 : 8), false); }   /* 8192 wide */
 
 constexpr int FWD_BLOCKS = 2048;      // 8 blocks of 4 waves a CU
 constexpr int BWD_BLOCKS = 512;       // 2 a CU: each writes 8 C bytes of partial sums
@@ -269,10 +308,10 @@ template <typename T>
 int launch_fwd(const NormFwdParams& p, hipStream_t st) {
   const Shape s = pick((p.C + Elem<T>::VEC - 1) / Elem<T>::VEC);
   const dim3 grid((unsigned)blocks_for(p.R, s.lpr, FWD_BLOCKS));
-#define HI3D_L(LPR, NV)                                                                                               \
+#define HI3D_L(LPR, NV, TINY)                                                                                               \
   do {                                                                                                                \
-    if (p.r) hipLaunchKernelGGL((norm_fwd_kernel<T, LPR, NV, true>), grid, dim3(NTHR), 0, st, p);                     \
-    else hipLaunchKernelGGL((norm_fwd_kernel<T, LPR, NV, false>), grid, dim3(NTHR), 0, st, p);                        \
+    if (p.r) hipLaunchKernelGGL((norm_fwd_kernel<T, LPR, NV, true, TINY>), grid, dim3(NTHR), 0, st, p);                     \
+    else hipLaunchKernelGGL((norm_fwd_kernel<T, LPR, NV, false, TINY>), grid, dim3(NTHR), 0, st, p);                        \
   } while (0)
   HI3D_NORM_SHAPES(HI3D_L)
 #undef HI3D_L
@@ -284,7 +323,7 @@ template <typename T>
 int launch_bwd(const NormBwdParams& p, int nblk, hipStream_t st) {
   const Shape s = pick((p.C + Elem<T>::VEC - 1) / Elem<T>::VEC);
   const dim3 grid((unsigned)nblk);
-#define HI3D_L(LPR, NV) hipLaunchKernelGGL((norm_bwd_kernel<T, LPR, NV>), grid, dim3(NTHR), 0, st, p)
+#define HI3D_L(LPR, NV, TINY) hipLaunchKernelGGL((norm_bwd_kernel<T, LPR, NV, TINY>), grid, dim3(NTHR), 0, st, p)
   HI3D_NORM_SHAPES(HI3D_L)
 #undef HI3D_L
   HI3D_LAUNCH_CHECK();

@@ -1,10 +1,12 @@
 // What the training kernels share: element types, vector loads of any element alignment, sums over a group of lanes.
 #pragma once
 #include "common.h"
+#include <type_traits>
 
 namespace {
 
 typedef _Float16 half_t;
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 struct bf16_t { unsigned short u; };
 
 template <typename T> struct Elem;
@@ -24,36 +26,82 @@ template <> struct Elem<bf16_t> {
   static __device__ __forceinline__ bf16_t put(float v) { return bf16_t{f32_to_bf16(v)}; }
 };
 
-// N elements in one access.  The alignment asked for is the element's own: gfx950 takes global vector accesses at any byte
-// address (unaligned access mode), so views at odd offsets and rows of odd length use the same 16-byte loads.
+// N elements in one access, as raw 32-bit words.  The alignment asked for is the element's own: gfx950 takes global vector accesses at any
+// byte address (unaligned access mode), so views at odd offsets and rows of odd length use the same 16-byte loads.
 template <typename T, int N>
-struct __attribute__((packed, aligned(sizeof(T)))) Pack { T v[N]; };
+struct __attribute__((packed, aligned(sizeof(T)))) Pack {
+  static constexpr int W = N * (int)sizeof(T) / 4;
+  static_assert(W * 4 == N * (int)sizeof(T), "whole words");
+  unsigned w[W];
+};
 
-// The first n of N elements of a row's vector (n <= 0: none), the others zero, as raw bits: a full vector is one masked load whose
-// result nothing waits for until it is unpacked, so that a row's loads are all in flight together.
-template <typename T, int N>
-__device__ __forceinline__ void fetch(const T* p, int n, Pack<T, N>& k) {
-  k = Pack<T, N>{};
-  if (n >= N) k = *(const Pack<T, N>*)p;
-  else if (n > 0) {
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (j < n) k.v[j] = p[j];
-  }
-}
 template <typename T, int N>
 __device__ __forceinline__ void unpack(const Pack<T, N>& k, float (&f)[N]) {
 #pragma unroll
-  for (int j = 0; j < N; ++j) f[j] = Elem<T>::get(k.v[j]);
+  for (int j = 0; j < Pack<T, N>::W; ++j) {
+    if constexpr (sizeof(T) == 4) f[j] = __uint_as_float(k.w[j]);
+    else if constexpr (std::is_same<T, bf16_t>::value) { f[2 * j] = __uint_as_float(k.w[j] << 16); f[2 * j + 1] = __uint_as_float(k.w[j] & 0xffff0000u); }
+    else {
+      const half2_t h = __builtin_bit_cast(half2_t, k.w[j]);
+      f[2 * j] = (float)h[0]; f[2 * j + 1] = (float)h[1];
+    }
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> pack(const float (&f)[N]) {
+  Pack<T, N> k;
+#pragma unroll
+  for (int j = 0; j < Pack<T, N>::W; ++j) {
+    if constexpr (sizeof(T) == 4) k.w[j] = __float_as_uint(f[j]);
+    else if constexpr (std::is_same<T, bf16_t>::value) k.w[j] = pack_bf16x2(f[2 * j], f[2 * j + 1]);
+    else k.w[j] = __builtin_bit_cast(unsigned, half2_t{(half_t)f[2 * j], (half_t)f[2 * j + 1]});
+  }
+  return k;
+}
+// k moved down by s of its N elements (0 <= s < N), zeros behind
+template <typename T, int N>
+__device__ __forceinline__ void shift_down(Pack<T, N>& k, int s) {
+  constexpr int W = Pack<T, N>::W, PER = 4 / (int)sizeof(T);
+#pragma unroll
+  for (int step = W / 2; step > 0; step >>= 1) {
+    const bool on = s & (step * PER);
+#pragma unroll
+    for (int j = 0; j < W; ++j) k.w[j] = on ? (j + step < W ? k.w[j + step] : 0u) : k.w[j];
+  }
+  if constexpr (PER == 2) {
+    const bool on = s & 1;
+#pragma unroll
+    for (int j = 0; j < W; ++j) k.w[j] = on ? (k.w[j] >> 16) | (j + 1 < W ? k.w[j + 1] << 16 : 0u) : k.w[j];
+  }
+}
+// The first n of N elements at p (n <= 0: none), the others zero.  A vector that the row's end cuts is loaded so that it ends there, and moved down
+// afterwards: one access, nothing is read outside the row; `before` elements precede p in its row, and where those are too few the elements come one by one.
+template <typename T, int N>
+__device__ __forceinline__ void fetch(const T* p, int n, long before, Pack<T, N>& k) {
+#pragma unroll
+  for (int j = 0; j < Pack<T, N>::W; ++j) k.w[j] = 0;
+  if (n >= N) k = *(const Pack<T, N>*)p;
+  else if (n > 0) {
+    Pack<T, N> t = {};
+    if (before >= N - n) {
+      t = *(const Pack<T, N>*)(p - (N - n));
+      shift_down(t, N - n);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (j < n) {
+          if constexpr (sizeof(T) == 4) t.w[j] = *(const unsigned*)(p + j);
+          else t.w[j / 2] |= (unsigned)*(const unsigned short*)(p + j) << (16 * (j & 1));
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < Pack<T, N>::W; ++j) k.w[j] = t.w[j];
+  }
 }
 template <typename T, int N>
 __device__ __forceinline__ void store_some(T* p, int n, const float (&f)[N]) {
-  if (n >= N) {
-    Pack<T, N> k;
-#pragma unroll
-    for (int j = 0; j < N; ++j) k.v[j] = Elem<T>::put(f[j]);
-    *(Pack<T, N>*)p = k;
-  } else if (n > 0) {
+  if (n >= N) *(Pack<T, N>*)p = pack<T, N>(f);
+  else if (n > 0) {
 #pragma unroll
     for (int j = 0; j < N; ++j)
       if (j < n) p[j] = Elem<T>::put(f[j]);
@@ -62,9 +110,9 @@ __device__ __forceinline__ void store_some(T* p, int n, const float (&f)[N]) {
 // elements [e, e + n) of a tensor whose type is known at run time only (weights: read once per block)
 template <int N>
 __device__ __forceinline__ void load_vec_as(const void* p, int code, int e, int n, float (&f)[N]) {
-  if (code == HI3D_F32) { Pack<float, N> k; fetch((const float*)p + e, n, k); unpack(k, f); }
-  else if (code == HI3D_BF16) { Pack<bf16_t, N> k; fetch((const bf16_t*)p + e, n, k); unpack(k, f); }
-  else { Pack<half_t, N> k; fetch((const half_t*)p + e, n, k); unpack(k, f); }
+  if (code == HI3D_F32) { Pack<float, N> k; fetch((const float*)p + e, n, e, k); unpack(k, f); }
+  else if (code == HI3D_BF16) { Pack<bf16_t, N> k; fetch((const bf16_t*)p + e, n, e, k); unpack(k, f); }
+  else { Pack<half_t, N> k; fetch((const half_t*)p + e, n, e, k); unpack(k, f); }
 }
 
 // one element of a tensor whose type is known at run time only (weights, biases: read or written once per block)
