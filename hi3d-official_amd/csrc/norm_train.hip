@@ -30,8 +30,6 @@ struct NormBwdParams {
   int C, wcode, want;       // want: partial sums of dw, db are asked for
 };
 
-constexpr int NTHR = 256;
-
 // A row's vectors as one lane holds them: vector i covers elements at[i] ... at[i] + V of the row, n[i] of which exist.  The one that the
 // row's end cuts is read so that it ends there and moved down once all of the row's loads are out (`settle`).  TINY: rows shorter than a
 // vector, element by element.
@@ -39,11 +37,11 @@ template <typename T, int LPR, int NV, bool TINY>
 struct RowMap {
   static constexpr int V = Elem<T>::VEC;
   int n[NV];
-  bool ragged;
+  int cut;                                // which of a lane's vectors the end of the row can cut; -1: none
   __device__ __forceinline__ RowMap(int l, int C) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) n[i] = C - (l + i * LPR) * V;
-    ragged = C % V != 0;
+    cut = C % V != 0 ? C / V / LPR : -1;
   }
   __device__ __forceinline__ void load(const T* row, int l, bool in, Pack<T, V> (&k)[NV]) const {
 #pragma unroll
@@ -58,11 +56,11 @@ struct RowMap {
     }
   }
   __device__ __forceinline__ void settle(Pack<T, V> (&k)[NV]) const {
-    if constexpr (!TINY)
-      if (ragged) {
+    if constexpr (!TINY) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) shift_down(k[i], n[i] > 0 && n[i] < V ? V - n[i] : 0);
-      }
+      for (int i = 0; i < NV; ++i)
+        if (i == cut) shift_down(k[i], n[i] > 0 && n[i] < V ? V - n[i] : 0);
+    }
   }
   // a weight or bias of the run-time type `code` in the lane's columns (1 or 0 where there is none)
   __device__ __forceinline__ void columns(const void* p, int code, int l, float none, float (&f)[NV][V]) const {
@@ -90,18 +88,23 @@ struct RowMap {
 template <int LPR>
 __device__ __forceinline__ float row_sum(float v, float* lds, int& slot) {
   if constexpr (LPR <= 64) return group_sum<LPR>(v);
+  constexpr int WAVES = LPR / 64;
   v = group_sum<64>(v);
-  float* s = lds + (slot & 1) * 4;
+  float* s = lds + (slot & 1) * WAVES;
   if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
   __syncthreads();
   ++slot;
-  return (s[0] + s[1]) + (s[2] + s[3]);
+  v = s[0];
+#pragma unroll
+  for (int k = 1; k < WAVES; ++k) v += s[k];
+  return v;
 }
+constexpr int threads_of(int lpr) { return lpr < 256 ? 256 : lpr; }
 
 template <typename T, int LPR, int NV, bool ADD, bool TINY>
-__global__ __launch_bounds__(NTHR) void norm_fwd_kernel(const NormFwdParams p) {
-  constexpr int V = Elem<T>::VEC, RPB = NTHR / LPR;
-  __shared__ float lds[8];
+__global__ __launch_bounds__(threads_of(LPR)) void norm_fwd_kernel(const NormFwdParams p) {
+  constexpr int V = Elem<T>::VEC, THR = threads_of(LPR), RPB = THR / LPR;
+  __shared__ float lds[2 * THR / 64];
   int slot = 0;
   const int l = threadIdx.x % LPR, sub = threadIdx.x / LPR, C = p.C;
   const RowMap<T, LPR, NV, TINY> map(l, C);
@@ -162,10 +165,11 @@ __global__ __launch_bounds__(NTHR) void norm_fwd_kernel(const NormFwdParams p) {
 // the gradients of a block's rows: dx, and -- where they are asked for -- the block's sums of dy h and dy, in columns held by
 // the lane through all of its rows: nothing is added atomically, the order of the sums is that of the rows
 template <typename T, int LPR, int NV, bool TINY>
-__global__ __launch_bounds__(NTHR) void norm_bwd_kernel(const NormBwdParams p) {
-  constexpr int V = Elem<T>::VEC, RPB = NTHR / LPR;
-  __shared__ float lds[8];
-  __shared__ float cols[LPR <= 64 ? 4 * LPR * V : 1];
+__global__ __launch_bounds__(threads_of(LPR)) void norm_bwd_kernel(const NormBwdParams p) {
+  constexpr int V = Elem<T>::VEC, THR = threads_of(LPR), RPB = THR / LPR;
+  __shared__ float lds[2 * THR / 64];
+  constexpr int WIDTH = LPR * NV * V;
+  __shared__ float cols[LPR <= 64 ? 8 * WIDTH : 1];            // [wave][weight, bias][column, as the lanes hold them]
   int slot = 0;
   const int l = threadIdx.x % LPR, sub = threadIdx.x / LPR, C = p.C;
   const RowMap<T, LPR, NV, TINY> map(l, C);
@@ -216,123 +220,141 @@ __global__ __launch_bounds__(NTHR) void norm_bwd_kernel(const NormBwdParams p) {
   }
   if (!p.want) return;
   // the lanes that held the same columns: over the wave's row groups by shuffles, over the waves through LDS
-  float* part = p.part + (long)blockIdx.x * 2 * C;
+  float* const part = p.part + (long)blockIdx.x * 2 * C;
+  auto put = [&](int k, int e, float v) {
+    if (p.part) part[k * C + e] = v;
+    else if (k ? p.db : p.dw) store_as(k ? p.db : p.dw, p.wcode, e, v);
+  };
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      float t[V];
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        t[j] = k ? gb[i][j] : gw[i][j];
+        float t = k ? gb[i][j] : gw[i][j];
         if constexpr (LPR < 64) {
 #pragma unroll
-          for (int o = LPR; o < 64; o <<= 1) t[j] += __shfl_xor(t[j], o, 64);
+          for (int o = LPR; o < 64; o <<= 1) t += __shfl_xor(t, o, 64);
         }
+        if constexpr (LPR <= 64) {
+          if ((threadIdx.x & 63) < LPR) cols[((threadIdx.x >> 6) * 2 + k) * WIDTH + (i * V + j) * LPR + l] = t;
+        } else if (j < map.n[i]) put(k, (l + i * LPR) * V + j, t);
       }
-      if constexpr (LPR <= 64) {
-        const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-        __syncthreads();
-        if (lane < LPR) {
-#pragma unroll
-          for (int j = 0; j < V; ++j) cols[wv * LPR * V + l * V + j] = t[j];
-        }
-        __syncthreads();
-        for (int c = threadIdx.x; c < LPR * V; c += NTHR) {
-          const int e = i * LPR * V + c;
-          const float v = (cols[c] + cols[LPR * V + c]) + (cols[2 * LPR * V + c] + cols[3 * LPR * V + c]);
-          if (e < C) {
-            if (p.part) part[k * C + e] = v;
-            else if (k ? p.db : p.dw) store_as(k ? p.db : p.dw, p.wcode, e, v);
-          }
-        }
-      } else {
-        const int e = (l + i * LPR) * V;
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (j < map.n[i]) {
-            if (p.part) part[k * C + e + j] = t[j];
-            else if (k ? p.db : p.dw) store_as(k ? p.db : p.dw, p.wcode, e + j, t[j]);
-          }
-      }
+  if constexpr (LPR <= 64) {
+    __syncthreads();
+    for (int q = threadIdx.x; q < 2 * WIDTH; q += THR) {
+      const int k = q / WIDTH, s = q - k * WIDTH, ij = s / LPR, e = ((s - ij * LPR) + ij / V * LPR) * V + ij % V;
+      if (e < C) put(k, e, (cols[q] + cols[2 * WIDTH + q]) + (cols[4 * WIDTH + q] + cols[6 * WIDTH + q]));
     }
+  }
 }
 
-// out0 / out1[c] = sum over the nblk partial rows of part[blk][0 / 1][c] (a fixed order: the slices of a column in order, then the
-// slices' sums in order).  32 columns x 8 slices a block.
-__global__ __launch_bounds__(NTHR) void column_reduce_kernel(const float* part, void* o0, void* o1, int code0, int code1, int nblk, int C, int width) {
-  __shared__ float lds[8][33];
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + tx;
+// out0 / out1[c] = sum over the nblk partial rows of part[blk][0 / 1][c] in a fixed order: 64 slices of the rows, then two levels over the
+// slices.  16 columns a block: few columns have to make enough blocks, and a slice's loads are all in flight.
+__global__ __launch_bounds__(1024) void column_reduce_kernel(const float* part, void* o0, void* o1, int code0, int code1, int nblk, int C, int width) {
+  __shared__ float lds[64][17];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int c = blockIdx.x * 16 + tx;
   float s = 0.0f;
   if (c < width) {
-#pragma unroll 4
-    for (int b = ty; b < nblk; b += 8) s += part[(long)b * width + c];
+#pragma unroll 8
+    for (int b = ty; b < nblk; b += 64) s += part[(long)b * width + c];
   }
   lds[ty][tx] = s;
   __syncthreads();
-  if (ty == 0 && c < width) {
+  if (ty < 8) {
+    s = 0.0f;
 #pragma unroll
-    for (int k = 1; k < 8; ++k) s += lds[k][tx];
+    for (int k = 0; k < 8; ++k) s += lds[ty * 8 + k][tx];
+  }
+  __syncthreads();
+  if (ty < 8) lds[ty][tx] = s;
+  __syncthreads();
+  if (ty == 0 && c < width) {
+    s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += lds[k][tx];
     if (c < C) { if (o0) store_as(o0, code0, c, s); }
     else if (o1) store_as(o1, code1, c - C, s);
   }
 }
 
-// lanes per row and vectors per lane for a row of `chunks` vectors: the fewest lanes that hold it in at most 5 vectors each (more
-// rows per wave, fewer steps per sum), then the fewest vectors of the forms that are built
+// lanes per row and vectors per lane for a row of `chunks` vectors: the fewest lanes that hold it in at most `most` vectors each (more
+// rows per wave, fewer steps per sum), then the fewest vectors of the forms that are built.  Forward holds 5 vectors (320, 640 and 1280
+// columns of 16 bits fill 8, 16 and 32 lanes exactly); backward holds 3, since a lane also keeps its columns' sums: with 5 it had one wave
+// a SIMD (85 us for 65536 x 640 against 71).
 struct Shape { int lpr, nv; };
-Shape pick(int chunks) {
-  for (int lpr = 8; lpr <= 64; lpr *= 2)
-    if (chunks <= 5 * lpr) return {lpr, chunks <= 2 * lpr ? 2 : chunks <= 3 * lpr ? 3 : 5};
-  return {256, chunks <= 2 * 256 ? 2 : chunks <= 4 * 256 ? 4 : 8};
+Shape pick(int chunks, int most) {
+  for (int lpr = 8; ; lpr = lpr == 64 ? 256 : lpr * 2)
+    if (chunks <= most * lpr || lpr == 512) return {lpr, chunks <= 2 * lpr ? 2 : chunks <= 3 * lpr ? 3 : most < 5 ? 4 : 5};
 }
 
-#define HI3D_NORM_SHAPES(LAUNCH)                                                                                  \
-  if (p.C < Elem<T>::VEC) LAUNCH(8, 2, true); else                                                                                  \
-  if (s.lpr == 8) { if (s.nv == 2) LAUNCH(8, 2, false); else if (s.nv == 3) LAUNCH(8, 3, false); else LAUNCH(8, 5, false); }           \
-  else if (s.lpr == 16) { if (s.nv == 3) LAUNCH(16, 3, false); else if (s.nv == 2) LAUNCH(16, 2, false); else LAUNCH(16, 5, false); }  \
-  else if (s.lpr == 32) { if (s.nv == 3) LAUNCH(32, 3, false); else if (s.nv == 2) LAUNCH(32, 2, false); else LAUNCH(32, 5, false); }  \
-  else if (s.lpr == 64) { if (s.nv == 3) LAUNCH(64, 3, false); else if (s.nv == 2) LAUNCH(64, 2, false); else LAUNCH(64, 5, false); }  \
-  else { if (s.nv == 2) LAUNCH(256, 2, false); else if (s.nv == 4) LAUNCH(256, 4, false); else LAUNCH(256, (Elem<T>::VEC == 8 ? 4 : 8), false); }   /* 8192 wide */
+// whether pick() can give (lpr, nv) for a row of at most `chunks` vectors: what it cannot give is not built
+constexpr bool given(int lpr, int nv, int most, int chunks) {
+  const int before = lpr == 8 ? 0 : most * (lpr == 256 ? 64 : lpr / 2), fewer = nv == 2 ? 0 : nv == 3 ? 2 : 3;
+  const int lo = before > fewer * lpr ? before : fewer * lpr, hi = nv > most && lpr < 512 ? 0 : nv * lpr;
+  return lo < (hi < chunks ? hi : chunks);
+}
 
 constexpr int FWD_BLOCKS = 2048;      // 8 blocks of 4 waves a CU
-constexpr int BWD_BLOCKS = 512;       // 2 a CU: each writes 8 C bytes of partial sums
+constexpr int BWD_BLOCKS = 1024;      // each writes 8 C bytes of partial sums ...
+constexpr int BWD_ROWS = 4;           // ... so that few rows take fewer: this many for each group of lanes
+constexpr int FWD_MOST = 5, BWD_MOST = 3;
 
-long blocks_for(long R, int lpr, long most) {
-  const long rpb = NTHR / lpr, n = (R + rpb - 1) / rpb;
+long blocks_for(long R, int lpr, long most, int each) {
+  const long rpb = (long)(threads_of(lpr) / lpr) * each, n = (R + rpb - 1) / rpb;
   return n < most ? n : most;
 }
 
+struct Launch { Shape s; unsigned grid; hipStream_t st; bool tiny; };
+
+template <typename T, int LPR, int NV, bool TINY>
+bool fwd_as(const NormFwdParams& p, const Launch& q) {
+  if constexpr (TINY || given(LPR, NV, FWD_MOST, HI3D_NORM_MAX_WIDTH / Elem<T>::VEC)) {
+    if (TINY ? !q.tiny : q.s.lpr != LPR || q.s.nv != NV) return false;
+    if (p.r) hipLaunchKernelGGL((norm_fwd_kernel<T, LPR, NV, true, TINY>), dim3(q.grid), dim3(threads_of(LPR)), 0, q.st, p);
+    else hipLaunchKernelGGL((norm_fwd_kernel<T, LPR, NV, false, TINY>), dim3(q.grid), dim3(threads_of(LPR)), 0, q.st, p);
+    return true;
+  }
+  return false;
+}
+template <typename T, int LPR, int NV, bool TINY>
+bool bwd_as(const NormBwdParams& p, const Launch& q) {
+  if constexpr (TINY || given(LPR, NV, BWD_MOST, HI3D_NORM_MAX_WIDTH / Elem<T>::VEC)) {
+    if (TINY ? !q.tiny : q.s.lpr != LPR || q.s.nv != NV) return false;
+    hipLaunchKernelGGL((norm_bwd_kernel<T, LPR, NV, TINY>), dim3(q.grid), dim3(threads_of(LPR)), 0, q.st, p);
+    return true;
+  }
+  return false;
+}
+template <typename T, int LPR>
+bool fwd_row(const NormFwdParams& p, const Launch& q) { return fwd_as<T, LPR, 2, false>(p, q) || fwd_as<T, LPR, 3, false>(p, q) || fwd_as<T, LPR, 5, false>(p, q); }
+template <typename T, int LPR>
+bool bwd_row(const NormBwdParams& p, const Launch& q) { return bwd_as<T, LPR, 2, false>(p, q) || bwd_as<T, LPR, 3, false>(p, q); }
+
 template <typename T>
 int launch_fwd(const NormFwdParams& p, hipStream_t st) {
-  const Shape s = pick((p.C + Elem<T>::VEC - 1) / Elem<T>::VEC);
-  const dim3 grid((unsigned)blocks_for(p.R, s.lpr, FWD_BLOCKS));
-#define HI3D_L(LPR, NV, TINY)                                                                                               \
-  do {                                                                                                                \
-    if (p.r) hipLaunchKernelGGL((norm_fwd_kernel<T, LPR, NV, true, TINY>), grid, dim3(NTHR), 0, st, p);                     \
-    else hipLaunchKernelGGL((norm_fwd_kernel<T, LPR, NV, false, TINY>), grid, dim3(NTHR), 0, st, p);                        \
-  } while (0)
-  HI3D_NORM_SHAPES(HI3D_L)
-#undef HI3D_L
+  const Shape s = pick((p.C + Elem<T>::VEC - 1) / Elem<T>::VEC, FWD_MOST);
+  const Launch q = {s, (unsigned)blocks_for(p.R, s.lpr, FWD_BLOCKS, 1), st, p.C < Elem<T>::VEC};
+  const bool done = fwd_as<T, 8, 2, true>(p, q) || fwd_row<T, 8>(p, q) || fwd_row<T, 16>(p, q) || fwd_row<T, 32>(p, q) || fwd_row<T, 64>(p, q) || fwd_row<T, 256>(p, q) ||
+                    fwd_row<T, 512>(p, q);
+  if (!done) HI3D_FAIL(HI3D_ESHAPE, "layernorm_fwd: no kernel holds a row of this width");
   HI3D_LAUNCH_CHECK();
   return 0;
 }
-
 template <typename T>
 int launch_bwd(const NormBwdParams& p, int nblk, hipStream_t st) {
-  const Shape s = pick((p.C + Elem<T>::VEC - 1) / Elem<T>::VEC);
-  const dim3 grid((unsigned)nblk);
-#define HI3D_L(LPR, NV, TINY) hipLaunchKernelGGL((norm_bwd_kernel<T, LPR, NV, TINY>), grid, dim3(NTHR), 0, st, p)
-  HI3D_NORM_SHAPES(HI3D_L)
-#undef HI3D_L
+  const Launch q = {pick((p.C + Elem<T>::VEC - 1) / Elem<T>::VEC, BWD_MOST), (unsigned)nblk, st, p.C < Elem<T>::VEC};
+  const bool done = bwd_as<T, 8, 2, true>(p, q) || bwd_row<T, 8>(p, q) || bwd_row<T, 16>(p, q) || bwd_row<T, 32>(p, q) || bwd_row<T, 64>(p, q) || bwd_row<T, 256>(p, q) ||
+                    bwd_row<T, 512>(p, q) || bwd_as<T, 512, 4, false>(p, q);
+  if (!done) HI3D_FAIL(HI3D_ESHAPE, "layernorm_bwd: no kernel holds a row of this width");
   HI3D_LAUNCH_CHECK();
   return 0;
 }
 
 int bwd_blocks(long R, int C, int dtype) {
   const int vec = dtype == HI3D_F32 ? 4 : 8;
-  return (int)blocks_for(R, pick((C + vec - 1) / vec).lpr, BWD_BLOCKS);
+  return (int)blocks_for(R, pick((C + vec - 1) / vec, BWD_MOST).lpr, BWD_BLOCKS, BWD_ROWS);
 }
 
 int bad_sizes(const char* what, long R, int C, int dtype, int wcode) {
@@ -345,7 +367,7 @@ int bad_sizes(const char* what, long R, int C, int dtype, int wcode) {
 }  // namespace
 
 int hi3d_column_reduce(const float* part, void* o0, void* o1, int code0, int code1, int nblk, int C, int width, hipStream_t st) {
-  hipLaunchKernelGGL(column_reduce_kernel, dim3((width + 31) / 32), dim3(NTHR), 0, st, part, o0, o1, code0, code1, nblk, C, width);
+  hipLaunchKernelGGL(column_reduce_kernel, dim3((width + 15) / 16), dim3(1024), 0, st, part, o0, o1, code0, code1, nblk, C, width);
   HI3D_LAUNCH_CHECK();
   return 0;
 }

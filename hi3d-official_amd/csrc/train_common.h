@@ -127,11 +127,29 @@ __device__ __forceinline__ void store_as(void* p, int code, long i, float v) {
   else ((half_t*)p)[i] = (half_t)v;
 }
 
-// the sum of v over the aligned group of L lanes that this lane is in, in every one of them
+// The sum of v over the aligned group of L lanes that this lane is in, in every one of them: lane exchanges inside the vector unit (quad
+// permutations, mirrors of 8 and 16 lanes, swaps of rows and of halves), no LDS round trip.
+template <int CTRL>
+__device__ __forceinline__ float plus_dpp(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
+}
 template <int L>
 __device__ __forceinline__ float group_sum(float v) {
-#pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  static_assert(L == 8 || L == 16 || L == 32 || L == 64, "lanes of a row");
+  v = plus_dpp<0xB1>(v);                       // lane ^ 1
+  v = plus_dpp<0x4E>(v);                       // lane ^ 2
+  v = plus_dpp<0x141>(v);                      // the other four of 8
+  if constexpr (L >= 16) v = plus_dpp<0x140>(v);
+  if constexpr (L >= 32) {
+    const unsigned u = __float_as_uint(v);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  if constexpr (L >= 64) {
+    const unsigned u = __float_as_uint(v);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
   return v;
 }
 
