@@ -220,31 +220,41 @@ __global__ __launch_bounds__(threads_of(LPR)) void norm_bwd_kernel(const NormBwd
   }
   if (!p.want) return;
   // the lanes that held the same columns: over the wave's row groups by shuffles, over the waves through LDS
+  // (written in the order of the columns: whole lines)
   float* const part = p.part + (long)blockIdx.x * 2 * C;
-  auto put = [&](int k, int e, float v) {
-    if (p.part) part[k * C + e] = v;
-    else if (k ? p.db : p.dw) store_as(k ? p.db : p.dw, p.wcode, e, v);
-  };
+  void* const out[2] = {p.dw, p.db};
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int k = 0; k < 2; ++k) {
+      float t[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        float t = k ? gb[i][j] : gw[i][j];
+        t[j] = k ? gb[i][j] : gw[i][j];
         if constexpr (LPR < 64) {
 #pragma unroll
-          for (int o = LPR; o < 64; o <<= 1) t += __shfl_xor(t, o, 64);
+          for (int o = LPR; o < 64; o <<= 1) t[j] += __shfl_xor(t[j], o, 64);
         }
-        if constexpr (LPR <= 64) {
-          if ((threadIdx.x & 63) < LPR) cols[((threadIdx.x >> 6) * 2 + k) * WIDTH + (i * V + j) * LPR + l] = t;
-        } else if (j < map.n[i]) put(k, (l + i * LPR) * V + j, t);
+        if constexpr (LPR <= 64)
+          if ((threadIdx.x & 63) < LPR) cols[((threadIdx.x >> 6) * 2 + k) * WIDTH + (i * V + j) * LPR + l] = t[j];
       }
+      if constexpr (LPR > 64) {
+        const int e = (l + i * LPR) * V;
+        if (p.part) store_some(part + k * C + e, map.n[i], t);
+        else if (out[k]) {
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            if (j < map.n[i]) store_as(out[k], p.wcode, e + j, t[j]);
+        }
+      }
+    }
   if constexpr (LPR <= 64) {
     __syncthreads();
-    for (int q = threadIdx.x; q < 2 * WIDTH; q += THR) {
-      const int k = q / WIDTH, s = q - k * WIDTH, ij = s / LPR, e = ((s - ij * LPR) + ij / V * LPR) * V + ij % V;
-      if (e < C) put(k, e, (cols[q] + cols[2 * WIDTH + q]) + (cols[4 * WIDTH + q] + cols[6 * WIDTH + q]));
+    for (int q = threadIdx.x; q < 2 * C; q += THR) {
+      const int k = q >= C, e = q - k * C, vec = e / V, i = vec / LPR, s = k * WIDTH + (i * V + e % V) * LPR + vec % LPR;
+      const float v = (cols[s] + cols[2 * WIDTH + s]) + (cols[4 * WIDTH + s] + cols[6 * WIDTH + s]);
+      if (p.part) part[q] = v;
+      else if (out[k]) store_as(out[k], p.wcode, e, v);
     }
   }
 }
@@ -297,8 +307,11 @@ constexpr bool given(int lpr, int nv, int most, int chunks) {
 }
 
 constexpr int FWD_BLOCKS = 2048;      // 8 blocks of 4 waves a CU
-constexpr int BWD_BLOCKS = 1024;      // each writes 8 C bytes of partial sums ...
-constexpr int BWD_ROWS = 4;           // ... so that few rows take fewer: this many for each group of lanes
+// Backward, two blocks of 4 waves a CU (registers allow no more).  A block ends with 8 C bytes of partial sums, so that few rows take
+// fewer blocks: 4 rows for each group of lanes, 8 where a row takes the block (7013 x 1280 bf16: 1, 2, 4, 8, 16 rows 27, 27, 21, 24, 33 us;
+// 2000 x 5120: 37, 37, 29, 28, 37 us)
+constexpr int BWD_BLOCKS = 512;
+constexpr int bwd_rows(int lpr) { return lpr < 256 ? 4 : 8; }
 constexpr int FWD_MOST = 5, BWD_MOST = 3;
 
 long blocks_for(long R, int lpr, long most, int each) {
@@ -354,7 +367,8 @@ int launch_bwd(const NormBwdParams& p, int nblk, hipStream_t st) {
 
 int bwd_blocks(long R, int C, int dtype) {
   const int vec = dtype == HI3D_F32 ? 4 : 8;
-  return (int)blocks_for(R, pick((C + vec - 1) / vec, BWD_MOST).lpr, BWD_BLOCKS, BWD_ROWS);
+  const int lpr = pick((C + vec - 1) / vec, BWD_MOST).lpr;
+  return (int)blocks_for(R, lpr, BWD_BLOCKS, bwd_rows(lpr));
 }
 
 int bad_sizes(const char* what, long R, int C, int dtype, int wcode) {
