@@ -330,6 +330,83 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mat_kernel(const MatParams p)
 #endif
 }
 
+// ---- few rows ---------------------------------------------------------------------------------------------------------------------
+// y for at most 16 MT rows of x: the weights are all there is to read, once.  A block takes 16 / CS columns of the output and its 16 waves a
+// 16th of the contraction each, straight from memory into matrix operands -- no LDS, no padded copies: any pitch and alignment -- with U
+// steps of 32 in flight; the waves' sums meet in LDS in the order of the waves.
+// CS > 1 (at most 16 / CS rows of x): the 16 rows of the matrix operand are 16 / CS columns of the output times CS pieces of the contraction,
+// those of the other operand rows of x times the same pieces, and of the product the entries of equal pieces are used: a long
+// contraction makes CS times the blocks (N = 1280, K = 5120, one row: 80 blocks 8.4 us, 160 blocks 6.3 us).
+// Rows behind M and columns behind N repeat the last one and are not stored.
+constexpr int FEW_WAVES = 16;
+struct FewParams { const void* x; const void* w; Epilogue e; long ldx, ldw; int M, N, K; };
+
+template <typename T, int MT, int CS>
+__global__ __launch_bounds__(FEW_WAVES * 64) void few_rows_kernel(const FewParams p) {
+#if __HIP_DEVICE_COMPILE__
+  constexpr int U = MT == 1 ? 8 : 4, COLS = 16 / CS, ROWS = 16 * MT / CS;
+  static_assert(MT == 1 || CS == 1, "pieces only where 16 rows are too many");
+  __shared__ __attribute__((aligned(16))) float sums[FEW_WAVES][16 * MT][16];
+  __shared__ float whole[ROWS][COLS];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, fg = lane >> 4;
+  const int n0 = blockIdx.x * COLS;
+  const int per = ((p.K + 31) / 32 + FEW_WAVES * CS - 1) / (FEW_WAVES * CS);          // steps of 32 of a piece
+  const int k0 = (w * CS + fr % CS) * per * 32 + fg * 8, last = (w * CS + CS - 1) * per * 32;       // this lane's; the wave's last piece's
+  const T* const wr = (const T*)p.w + (long)min(n0 + fr / CS, p.N - 1) * p.ldw;
+  const T* xr[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) xr[i] = (const T*)p.x + (long)min((i * 16 + fr) / CS, p.M - 1) * p.ldx;
+  f32x4 acc[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < per; s += U) {
+    Pack<T, 8> kw[U], kx[U][MT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + (s + u) * 32;
+      if (s + u >= per) continue;
+      if (last + (s + u + 1) * 32 <= p.K) {
+        kw[u] = *(const Pack<T, 8>*)(wr + k);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) kx[u][i] = *(const Pack<T, 8>*)(xr[i] + k);
+      } else {                                     // the contraction's end in some lanes
+        fetch(wr + k, p.K - k, k, kw[u]);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) fetch(xr[i] + k, p.K - k, k, kx[u][i]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s + u >= per) continue;
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+        acc[i] = Mfma<T>::mul(u32x4{kw[u].w[0], kw[u].w[1], kw[u].w[2], kw[u].w[3]}, u32x4{kx[u][i].w[0], kx[u][i].w[1], kx[u][i].w[2], kx[u][i].w[3]}, acc[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i) *(f32x4*)&sums[w][i * 16 + fr][fg * 4] = acc[i];
+  __syncthreads();
+  for (int q = threadIdx.x; q < ROWS * COLS; q += FEW_WAVES * 64) {
+    const int m = q / COLS, n = q % COLS;
+    float t = 0.0f;
+#pragma unroll
+    for (int k = 0; k < FEW_WAVES; ++k)
+#pragma unroll
+      for (int c = 0; c < CS; ++c) t += sums[k][m * CS + c][n * CS + c];
+    whole[m][n] = t;
+  }
+  __syncthreads();
+  constexpr int CHUNKS = (COLS + 7) / 8;
+  const int m = threadIdx.x / CHUNKS, c = (threadIdx.x % CHUNKS) * 8, n = min(COLS, p.N - n0) - c;
+  if (m < p.M && m < ROWS && n > 0) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c + j < COLS ? whole[m][c + j] : 0.0f;
+    finish<T>(p.e, m, n0 + c, n, v);
+  }
+#endif
+}
+
 // the partial sums of a split contraction, in the order of the splits, and the epilogue
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(const float* part, Epilogue e, long M, int N, int splits) {
@@ -338,6 +415,7 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, Epilogue e
     const long m = c / cpr;
     const int n = (int)(c - m * cpr) * 8;
     float v[8] = {};
+#pragma unroll 4
     for (int s = 0; s < splits; ++s) {
       Pack<float, 8> k;
       fetch(part + (s * M + m) * N + n, N - n, n, k);
@@ -510,8 +588,28 @@ bool too_big(const hi3d_linear_desc* d) {
          (d->M > 1 && (d->ldx > most || d->lddy > most || d->ldz > (1L << 40) || d->ldr > (1L << 40))) || (d->N > 1 && d->ldw > most);
 }
 
+// Up to 32 rows the weights are streamed by few_rows_kernel, above that the tiles are faster (N = K = 4096, 32 / 48 / 65 rows: streamed 14 /
+// 19 us, tiles 18 us for up to 128).
+constexpr int FEW = 32;
+template <typename T, int MT, int CS>
+int launch_few(const FewParams& p, hipStream_t st) {
+  hipLaunchKernelGGL((few_rows_kernel<T, MT, CS>), dim3((p.N + 16 / CS - 1) / (16 / CS)), dim3(FEW_WAVES * 64), 0, st, p);
+  HI3D_LAUNCH_CHECK();
+  return 0;
+}
+template <typename T>
+int few_rows(const FewParams& p, hipStream_t st) {
+  // pieces of the contraction: as the rows leave room for them, while a wave keeps two steps of 32 and there are no more blocks than CUs (one
+  // row, N = 4096, K = 4096: 1, 2, 4 pieces 10, 12, 15 us)
+  if (p.M > 16) return launch_few<T, 2, 1>(p, st);
+  if (p.M <= 4 && p.K >= 4 * FEW_WAVES * 64 && p.N <= 4 * CUS) return launch_few<T, 1, 4>(p, st);
+  if (p.M <= 8 && p.K >= 2 * FEW_WAVES * 64 && p.N <= 8 * CUS) return launch_few<T, 1, 2>(p, st);
+  return launch_few<T, 1, 1>(p, st);
+}
+
 struct FwdNeeds { long x, w, part; Plan plan; };
 FwdNeeds fwd_needs(const hi3d_linear_desc* d) {
+  if (d->M <= FEW) return {};
   FwdNeeds n = {0, 0, 0, plan_of(d->M, d->N, d->K)};
   if (!in_place(d->x, d->ldx, d->K)) n.x = padded_bytes(d->M, d->K);
   if (!in_place(d->w, d->ldw, d->K)) n.w = padded_bytes(d->N, d->K);
@@ -535,6 +633,11 @@ BwdNeeds bwd_needs(const hi3d_linear_desc* d) {
 
 template <typename T>
 int fwd(const hi3d_linear_desc* d, hipStream_t st) {
+  const Epilogue e = {d->bias, d->residual, d->y, d->z, (long)d->ldr, (long)d->N, d->bias_dtype, d->act};
+  if (d->M <= FEW) {
+    const FewParams p = {d->x, d->w, e, (long)d->ldx, (long)d->ldw, (int)d->M, d->N, d->K};
+    return few_rows<T>(p, st);
+  }
   const FwdNeeds n = fwd_needs(d);
   char* ws = (char*)d->ws;
   Operand x, w;
@@ -543,7 +646,7 @@ int fwd(const hi3d_linear_desc* d, hipStream_t st) {
   MatParams p = {};
   p.A = (const char*)x.p; p.B = (const char*)w.p; p.lda = x.ld; p.ldb = w.ld;
   p.M = (int)d->M; p.N = d->N; p.K = d->K;
-  p.e = {d->bias, d->residual, d->y, d->z, (long)d->ldr, (long)d->N, d->bias_dtype, d->act};
+  p.e = e;
   return launch_mat<T, false, false>(p, n.plan, (float*)ws, st);
 }
 
