@@ -278,28 +278,65 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mat_kernel(const MatParams p)
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   const int steps = (p.K + BK - 1) / BK, kb = ks * p.per, ke = min(steps, kb + p.per);
-  ta.issue(kb, smem, w);
-  tb.issue(kb, smem + ABYTES, w);
-  for (int kt = kb; kt < ke; ++kt) {
-    char* const s = smem + ((kt - kb) & 1) * STAGE;
+  u32x4 a[MT], b[NT];
+  auto issue = [&](int kt) {
+    char* const d = smem + ((kt - kb) & 1) * STAGE;
+    ta.issue(kt, d, w);
+    tb.issue(kt, d + ABYTES, w);
+  };
+  auto read = [&](const char* s, auto kh) {
+    fa.template read<decltype(kh)::value>(s, a, lane);
+    fb.template read<decltype(kh)::value>(s + ABYTES, b, lane);
+  };
+  auto multiply = [&]() {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) acc[i][j] = Mfma<T>::mul(b[j], a[i], acc[i][j]);
+  };
+  issue(kb);
+  if constexpr (NW == 8) {
+    // Two waves a SIMD, half a phase apart: a phase is [LDS-DMA of the next tile, fragment reads] barrier [matrix instructions] barrier, and
+    // waves 4 ... 7 are one barrier behind, so that of the two waves on a SIMD one reads while the other multiplies.  The next tile goes
+    // over the one that step kt - 1 read: its last fragment reads had returned (lgkmcnt(0)) before the barrier that ended their segment,
+    // and the first wave to issue is one barrier further.  It is waited for in the step's last read segment; the trailing waves do so one
+    // barrier before the leading ones read it.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();                              // tile kt is there, and everyone is done with the other one
-    if (kt + 1 < ke) {
-      char* const d = smem + ((kt + 1 - kb) & 1) * STAGE;
-      ta.issue(kt + 1, d, w);
-      tb.issue(kt + 1, d + ABYTES, w);
-    }
-    u32x4 a[MT], b[NT];
-    auto half = [&](auto kh) {
-      fa.template read<decltype(kh)::value>(s, a, lane);
-      fb.template read<decltype(kh)::value>(s + ABYTES, b, lane);
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = Mfma<T>::mul(b[j], a[i], acc[i][j]);
+    __builtin_amdgcn_s_barrier();
+    if (w >= 4) __builtin_amdgcn_s_barrier();
+    auto phase = [&](const char* s, auto kh) {
+      constexpr bool LAST = decltype(kh)::value == 1;
+      read(s, kh);
+      if (LAST) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);
+      multiply();
+      __builtin_amdgcn_s_setprio(0);
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
     };
-    half(std::integral_constant<int, 0>{});
-    half(std::integral_constant<int, 1>{});
+    for (int kt = kb; kt < ke; ++kt) {
+      const char* const s = smem + ((kt - kb) & 1) * STAGE;
+      if (kt + 1 < ke) issue(kt + 1);
+      phase(s, std::integral_constant<int, 0>{});
+      phase(s, std::integral_constant<int, 1>{});
+    }
+    if (w < 4) __builtin_amdgcn_s_barrier();
+  } else {
+    for (int kt = kb; kt < ke; ++kt) {
+      const char* const s = smem + ((kt - kb) & 1) * STAGE;
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();                              // tile kt is there, and everyone is done with the other one
+      if (kt + 1 < ke) issue(kt + 1);
+      read(s, std::integral_constant<int, 0>{});
+      multiply();
+      read(s, std::integral_constant<int, 1>{});
+      multiply();
+    }
   }
   __syncthreads();                                // the tiles' LDS is free
 
