@@ -295,6 +295,13 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mat_kernel(const MatParams p)
       for (int j = 0; j < NT; ++j) acc[i][j] = Mfma<T>::mul(b[j], a[i], acc[i][j]);
   };
   issue(kb);
+  if (threadIdx.x < BN / 8) {                       // the bias of the tile's columns (zeros where there is none) behind the tiles
+    float f[8] = {};
+    const int c = threadIdx.x * 8;
+    if (!p.part && p.e.bias) load_vec_as(p.e.bias, p.e.bcode, n0 + c, p.N - n0 - c, f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ((float*)(smem + 2 * STAGE))[c + j] = f[j];
+  }
   if constexpr (NW == 8) {
     // Two waves a SIMD, half a phase apart: a phase is [LDS-DMA of the next tile, fragment reads] barrier [matrix instructions] barrier, and
     // waves 4 ... 7 are one barrier behind, so that of the two waves on a SIMD one reads while the other multiplies.  The next tile goes
@@ -340,29 +347,146 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mat_kernel(const MatParams p)
   }
   __syncthreads();                                // the tiles' LDS is free
 
-  // each wave turns its accumulators 16 rows at a time into whole rows, in a slab of its own, and finishes 8 columns a lane
-  constexpr int WCOLS = 16 * NT, ROW = WCOLS * 4 + 16, CPR = WCOLS / 8;
-  static_assert(NW * 16 * ROW <= 2 * STAGE, "slabs fit the tiles' LDS");
-  char* const slab = smem + w * 16 * ROW;
+  // Bias and activation are taken where the accumulators are; the results leave in whole rows of the tile (a wave's own columns are 160 bytes of a
+  // row, and lines that several waves write a part of at different times cost a 65536 x 2560 output 60 us of 353), 16 rows of every wave row at a
+  // time through LDS: rounded values, or fp32 where a residual or other partial sums are still to be added.  Two buffers in turn, so that one
+  // barrier per pass is enough -- a buffer is written again two passes on, behind a barrier that its readers have passed.  Stores and residual
+  // loads go through buffer descriptors: what lies outside is dropped there, without a branch for the compiler to wait at.
+  //   rounded: pitch 2 BN + 16 bytes, 8 bytes a lane and column block: 32 lanes fall on all 64 banks.
+  //   fp32: pitch 4 BN + 16 bytes, the 16-byte units of a row even ones first: a thread's two units are read by two accesses whose lanes lie
+  //   side by side (side by side in the row, each access had half the banks).
+  constexpr int SROWS = 16 * WM, CPR = BN / 8, TH = NW * 64, CH = (SROWS * CPR + TH - 1) / TH;
+  constexpr int FROW = BN * 4 + 16, HROW = BN * 2 + 16, FSLAB = SROWS * FROW, HSLAB = SROWS * HROW;
+  static_assert(2 * (FSLAB + HSLAB) <= 2 * STAGE, "two buffers of both kinds fit the tiles' LDS");
+  constexpr unsigned NONE = 0x80000000u;
   const int fr = lane & 15, fg = lane >> 4;
+  const int cols = p.N - n0;                        // of the tile that exist
+  const bool fits = p.N % 8 == 0 && (!p.e.res || (p.e.ldr % 8 == 0 && ((unsigned long)p.e.res & 15) == 0));      // 16-byte accesses do
+  const bool wide = p.part || p.e.res || !fits;     // fp32 through LDS
+  const int wrow = wm * 16 + fr, wcol = wn * 16 * NT + fg * 4;
+  f32x4 bias[NT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
+  for (int j = 0; j < NT; ++j) bias[j] = *(const f32x4*)(smem + 2 * STAGE + (wcol + j * 16) * 4);
+  const int esz = p.part ? 4 : 2;
+  const long ldo = p.part ? p.N : p.e.ldo;
+  unsigned off[CH], roff[CH];                       // of the thread's chunks of 8 columns: bytes in the output and the residual, the LDS places
+  int hat[CH], fat[CH];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) *(f32x4*)(slab + fr * ROW + (j * 16 + fg * 4) * 4) = acc[i][j];
-    __builtin_amdgcn_wave_barrier();
+  for (int t = 0; t < CH; ++t) {
+    const int c = t * TH + threadIdx.x, r = c / CPR, q = c - r * CPR, row = (r >> 4) * 16 * MT + (r & 15);
+    const bool in = c < SROWS * CPR && q * 8 < cols;
+    hat[t] = in ? r * HROW + q * 16 : 0;
+    fat[t] = in ? r * FROW + q * 16 : 0;
+    off[t] = in ? (unsigned)((row * (int)ldo + q * 8) * esz) : NONE;
+    roff[t] = in ? (unsigned)((row * (int)p.e.ldr + q * 8) * 2) : NONE;
+  }
+  auto window = [&](const void* base, long ld, int size, int i) {        // rows m0 + 16 i ... of a matrix of M rows, from column n0
+    const long rows = p.M - m0 - 16 * i, valid = rows > 0 ? ((rows - 1) * ld + cols) * size : 0;
+    return __builtin_amdgcn_make_buffer_rsrc((char*)base + ((m0 + 16L * i) * ld + n0) * size, 0, (int)(valid > 0x7ffffff0 ? 0x7ffffff0 : valid), 0x00020000);
+  };
+  auto meet = [&]() {                               // this pass's rows are in LDS for everyone; outstanding stores are not waited for
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  auto to_fp32 = [&](char* slab, int j, const f32x4& v) {
+    const int u = (wcol + j * 16) >> 2;
+    *(f32x4*)(slab + wrow * FROW + ((u >> 1) + (u & 1) * CPR) * 16) = v;
+  };
+  auto to_rounded = [&](char* slab, int j, const f32x4& v) {
+    const float f[4] = {v[0], v[1], v[2], v[3]};
+    const Pack<T, 4> k = pack<T, 4>(f);
+    *(u32x2*)(slab + wrow * HROW + (wcol + j * 16) * 2) = u32x2{k.w[0], k.w[1]};
+  };
+  u32x4 res[CH];
+  auto residual = [&](int i) {
+    const __amdgpu_buffer_rsrc_t from = window(p.e.res, p.e.ldr, 2, i);
 #pragma unroll
-    for (int t = 0; t < (16 * CPR + 63) / 64; ++t) {
-      const int c = t * 64 + lane, row = c / CPR, col = (c - row * CPR) * 8;
-      const long m = m0 + wm * 16 * MT + i * 16 + row;
-      const int n = n0 + wn * WCOLS + col;
-      if (c < 16 * CPR && m < p.M && n < p.N) {
-        const f32x4 lo = *(const f32x4*)(slab + row * ROW + col * 4), hi = *(const f32x4*)(slab + row * ROW + col * 4 + 16);
-        float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        if (p.part) store_some(p.part + ((long)ks * p.M + m) * p.N + n, p.N - n, v);
-        else finish<T>(p.e, m, n, p.N - n, v);
+    for (int t = 0; t < CH; ++t) res[t] = __builtin_amdgcn_raw_buffer_load_b128(from, roff[t], 0, 0);
+  };
+  // WIDE: fp32 slabs;  ACT: the activation, or -1 where `finish` takes it (chunks that 16-byte accesses do not fit) or there is nothing to take
+  auto passes = [&](auto act_, auto wide_) {
+    constexpr int ACT = decltype(act_)::value;
+    constexpr bool WIDE = decltype(wide_)::value;
+    if (WIDE && ACT >= 0) residual(0);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      char* const fslab = smem + (i & 1) * FSLAB;
+      char* const hslab = smem + 2 * FSLAB + (i & 1) * HSLAB;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        f32x4 v = acc[i][j];
+        if constexpr (ACT >= 0) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] += bias[j][k];
+          if (p.e.z) to_rounded(WIDE ? hslab : fslab, j, v);
+          float f[4] = {v[0], v[1], v[2], v[3]};
+          activate(ACT, f);
+          v = f32x4{f[0], f[1], f[2], f[3]};
+        }
+        if (WIDE) to_fp32(fslab, j, v);
+        else to_rounded(hslab, j, v);
+      }
+      meet();
+      if constexpr (ACT < 0) {
+        if (p.part && p.N % 8 == 0) {
+          const __amdgpu_buffer_rsrc_t to = window(p.part + (long)ks * p.M * p.N, ldo, 4, i);
+#pragma unroll
+          for (int t = 0; t < CH; ++t) {
+            __builtin_amdgcn_raw_buffer_store_b128(*(const u32x4*)(fslab + fat[t]), to, off[t], 0, 0);
+            __builtin_amdgcn_raw_buffer_store_b128(*(const u32x4*)(fslab + fat[t] + CPR * 16), to, off[t] + 16, 0, 0);
+          }
+        } else {
+#pragma unroll 1
+          for (int c = threadIdx.x; c < SROWS * CPR; c += TH) {
+            const int r = c / CPR, q = c - r * CPR, n = n0 + q * 8;
+            const long m = m0 + (r >> 4) * 16 * MT + (r & 15) + i * 16;
+            if (m >= p.M || q * 8 >= cols) continue;
+            const f32x4 lo = *(const f32x4*)(fslab + r * FROW + q * 16), hi = *(const f32x4*)(fslab + r * FROW + q * 16 + CPR * 16);
+            float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            if (p.part) store_some(p.part + ((long)ks * p.M + m) * p.N + n, p.N - n, v);
+            else finish<T>(p.e, m, n, p.N - n, v);
+          }
+        }
+      } else {
+        if (p.e.z) {
+          const __amdgpu_buffer_rsrc_t to = window(p.e.z, ldo, 2, i);
+#pragma unroll
+          for (int t = 0; t < CH; ++t) __builtin_amdgcn_raw_buffer_store_b128(*(const u32x4*)((WIDE ? hslab : fslab) + hat[t]), to, off[t], 0, 0);
+        }
+        const __amdgpu_buffer_rsrc_t to = window(p.e.y, ldo, 2, i);
+        u32x4 y[CH];
+#pragma unroll
+        for (int t = 0; t < CH; ++t) {
+          if constexpr (WIDE) {
+            const f32x4 lo = *(const f32x4*)(fslab + fat[t]), hi = *(const f32x4*)(fslab + fat[t] + CPR * 16);
+            const Pack<T, 8> k = {{res[t][0], res[t][1], res[t][2], res[t][3]}};
+            float r[8];
+            unpack(k, r);
+            const float v[8] = {r[0] + lo[0], r[1] + lo[1], r[2] + lo[2], r[3] + lo[3], r[4] + hi[0], r[5] + hi[1], r[6] + hi[2], r[7] + hi[3]};
+            const Pack<T, 8> o = pack<T, 8>(v);
+            y[t] = u32x4{o.w[0], o.w[1], o.w[2], o.w[3]};
+          } else y[t] = *(const u32x4*)(hslab + hat[t]);
+        }
+        if (WIDE && i + 1 < MT) residual(i + 1);
+#pragma unroll
+        for (int t = 0; t < CH; ++t) __builtin_amdgcn_raw_buffer_store_b128(y[t], to, off[t], 0, 0);
       }
     }
-    __builtin_amdgcn_wave_barrier();
+  };
+  auto with = [&](auto act) {
+    if (wide) passes(act, std::true_type{});
+    else passes(act, std::false_type{});
+  };
+  using std::integral_constant;
+  if (p.part || !fits) passes(integral_constant<int, -1>{}, std::true_type{});
+  else if constexpr (AKS || BKS) passes(integral_constant<int, HI3D_ACT_NONE>{}, std::false_type{});       // a gradient: no epilogue
+  else switch (p.e.act) {
+    case HI3D_ACT_NONE: with(integral_constant<int, HI3D_ACT_NONE>{}); break;
+    case HI3D_ACT_GELU: with(integral_constant<int, HI3D_ACT_GELU>{}); break;
+    case HI3D_ACT_RELU: with(integral_constant<int, HI3D_ACT_RELU>{}); break;
+    case HI3D_ACT_SILU: with(integral_constant<int, HI3D_ACT_SILU>{}); break;
+    default: with(integral_constant<int, HI3D_ACT_QUICK_GELU>{}); break;
   }
 #endif
 }
@@ -554,7 +678,7 @@ long part_bytes(const Plan& p, long M, long N) { return p.splits > 1 ? round256(
 
 template <typename T, bool AKS, bool BKS, int WM, int WN, int MT, int NT>
 int launch_cfg(const MatParams& p, hipStream_t st) {
-  constexpr int LDS = 2 * (16 * MT * WM + 16 * NT * WN) * 128;
+  constexpr int LDS = 2 * (16 * MT * WM + 16 * NT * WN) * 128 + 16 * NT * WN * 4;        // two tiles, the bias
   static bool done[HI3D_MAX_DEVICES];
   if (const int rc = hi3d_raise_lds_limit((const void*)mat_kernel<T, AKS, BKS, WM, WN, MT, NT>, LDS, done)) return rc;
   hipLaunchKernelGGL((mat_kernel<T, AKS, BKS, WM, WN, MT, NT>), dim3((unsigned)(p.nbm * p.nbn * p.splits)), dim3(WM * WN * 64), LDS, st, p);
@@ -621,7 +745,7 @@ const char* bad_desc(const hi3d_linear_desc* d) {
 // tiles address their rows in 32 bits: 320 rows of 2 bytes an element
 bool too_big(const hi3d_linear_desc* d) {
   const long most = 0x7ffffff0L / 640;
-  return d->M > 0x7fff0000L || d->N > most || d->K > most || d->N > 0x200000 || d->K > 0x200000 ||
+  return d->M > 0x7fff0000L || d->N > most || d->K > most || d->N > 0x100000 || d->K > 0x100000 ||
          (d->M > 1 && (d->ldx > most || d->lddy > most || d->ldz > (1L << 40) || d->ldr > (1L << 40))) || (d->N > 1 && d->ldw > most);
 }
 
