@@ -201,8 +201,18 @@ struct Frags {
     } else {
       const unsigned b = (unsigned)(__UINTPTR_TYPE__)(LDS_AS const char*)lds;
 #pragma unroll
-      for (int t = 0; t < CNT; t += (CNT == 5 ? 5 : 4)) {
-        if constexpr (CNT == 5) {
+      for (int t = 0; t < CNT; t += (CNT == 5 ? 5 : CNT == 2 ? 2 : 4)) {
+        if constexpr (CNT == 2) {
+          u32x2 l0, l1, h0, h1;
+          asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%6\n\tds_read_b64_tr_b16 %2, %4 offset:%7\n\t"
+                       "ds_read_b64_tr_b16 %1, %5 offset:%6\n\tds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
+                       "s_waitcnt lgkmcnt(0)"
+                       : "=&v"(l0), "=&v"(l1), "=&v"(h0), "=&v"(h1)
+                       : "v"(b + addr[0]), "v"(b + addr[1]), "n"(KH * 4096), "n"(KH * 4096 + 1024)
+                       : "memory");
+          f[0] = u32x4{l0[0], l0[1], h0[0], h0[1]};
+          f[1] = u32x4{l1[0], l1[1], h1[0], h1[1]};
+        } else if constexpr (CNT == 5) {
           u32x2 l0, l1, l2, l3, l4, h0, h1, h2, h3, h4;
           asm volatile("ds_read_b64_tr_b16 %0, %10 offset:%15\n\tds_read_b64_tr_b16 %5, %10 offset:%16\n\t"
                        "ds_read_b64_tr_b16 %1, %11 offset:%15\n\tds_read_b64_tr_b16 %6, %11 offset:%16\n\t"
@@ -241,7 +251,7 @@ struct Frags {
 // WM x WN waves, each 16 MT x 16 NT of the output; two tiles of the contraction in LDS, the next one on its way while one is used.
 // The weight-side fragment is the first operand of the matrix instruction, so that a lane holds 4 consecutive columns of one output row.
 template <typename T, bool AKS, bool BKS, int WM, int WN, int MT, int NT>
-__global__ __launch_bounds__(WM * WN * 64, 2) void mat_kernel(const MatParams p) {
+__global__ __launch_bounds__(WM * WN * 64, MT == 2 ? 4 : 2) void mat_kernel(const MatParams p) {
 #if __HIP_DEVICE_COMPILE__
   constexpr int NW = WM * WN, BM = 16 * MT * WM, BN = 16 * NT * WN;
   constexpr int ABYTES = BM * 128, STAGE = (BM + BN) * 128;
@@ -647,27 +657,30 @@ __global__ __launch_bounds__(256) void slope_kernel(const SlopeParams p) {
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------------
-struct Config { int bm, bn, waves, slots; double step, fixed; };
-// step: us of one K step of a tile with the chip full, fixed: of a tile's start and end
-constexpr Config CONFIGS[] = {{256, 256, 8, 256, 1.75, 4.0}, {256, 320, 8, 256, 2.1, 4.5}, {128, 128, 4, 512, 1.1, 3.0}};
+// Tiles, and what one costs in us: a K step with one block on each CU and with `per_cu`, and a tile's start and end.  From sweeps of every tile and
+// split over M 65 ... 65536, N and K 320 ... 5120, all three products: what the estimate picks is within 10 % of the sweep's best nearly
+// everywhere.  64 x 64: small products whose blocks wait for memory and LDS rather than compute (2048 x 1024 x 1024: 14.8 -> 10.4 us).
+struct Config { int bm, bn, per_cu; double one, full, fixed; };
+constexpr Config CONFIGS[] = {{256, 256, 1, 1.45, 1.45, 10.0}, {256, 320, 1, 1.85, 1.85, 9.0}, {128, 128, 2, 0.85, 1.0, 4.0}, {64, 64, 4, 0.4, 0.65, 3.0}};
 constexpr int CUS = 256, MAX_SPLITS = 32;
 
-struct Plan { int cfg, splits, per; };
-// the tile and the split that the estimate above finds fastest
+struct Plan { int cfg, splits, per; double us; };
+// the tile and the split of the contraction that the estimate finds fastest: whole rounds of the chip, the rest at the occupancy that it
+// leaves, and the joining pass of a split
 Plan plan_of(long M, long N, long K) {
-  Plan best = {2, 1, 0};
-  double least = 1e300;
+  Plan best = {3, 1, 0, 1e300};
   const long steps = (K + BK - 1) / BK;
-  for (int c = 0; c < 3; ++c) {
+  for (int c = 0; c < 4; ++c) {
     const Config& f = CONFIGS[c];
-    const long tiles = ((M + f.bm - 1) / f.bm) * ((N + f.bn - 1) / f.bn);
+    const long tiles = ((M + f.bm - 1) / f.bm) * ((N + f.bn - 1) / f.bn), slots = (long)f.per_cu * CUS;
     for (long s = 1; s <= MAX_SPLITS && s <= steps; ++s) {
       const long per = (steps + s - 1) / s, splits = (steps + per - 1) / per;
       if (splits != s) continue;
-      if (s > 1 && tiles * s > 4 * f.slots) break;
-      const double waves = (double)((tiles * s + f.slots - 1) / f.slots);
-      const double t = waves * (per * f.step + f.fixed) + (s > 1 ? 4.0 + (double)M * N * (8.0 * s + 4.0) / 4.0e6 : 0.0);
-      if (t < least) { least = t; best = {c, (int)s, (int)per}; }
+      if (s > 1 && tiles * s > 4 * slots) break;
+      const long rounds = tiles * s / slots, rest = tiles * s % slots;
+      const double on_cu = rest > CUS ? (double)rest / CUS : 1.0, step = f.one + (f.per_cu > 1 ? (f.full - f.one) * (on_cu - 1.0) / (f.per_cu - 1) : 0.0);
+      const double us = rounds * (per * f.full + f.fixed) + (rest ? per * step + f.fixed : 0.0) + (s > 1 ? 4.5 + (double)M * N * (8.0 * s + 2.0) / 6.0e6 : 0.0);
+      if (us < best.us) best = {c, (int)s, (int)per, us};
     }
   }
   return best;
@@ -678,7 +691,7 @@ long part_bytes(const Plan& p, long M, long N) { return p.splits > 1 ? round256(
 
 template <typename T, bool AKS, bool BKS, int WM, int WN, int MT, int NT>
 int launch_cfg(const MatParams& p, hipStream_t st) {
-  constexpr int LDS = 2 * (16 * MT * WM + 16 * NT * WN) * 128 + 16 * NT * WN * 4;        // two tiles, the bias
+  constexpr int LDS = 2 * (16 * MT * WM + 16 * NT * WN) * 128 + 16 * NT * WN * 4;        // the tiles, the bias
   static bool done[HI3D_MAX_DEVICES];
   if (const int rc = hi3d_raise_lds_limit((const void*)mat_kernel<T, AKS, BKS, WM, WN, MT, NT>, LDS, done)) return rc;
   hipLaunchKernelGGL((mat_kernel<T, AKS, BKS, WM, WN, MT, NT>), dim3((unsigned)(p.nbm * p.nbn * p.splits)), dim3(WM * WN * 64), LDS, st, p);
@@ -696,7 +709,8 @@ int launch_mat(MatParams p, const Plan& plan, float* part, hipStream_t st) {
   int rc;
   if (plan.cfg == 0) rc = launch_cfg<T, AKS, BKS, 2, 4, 8, 4>(p, st);
   else if (plan.cfg == 1) rc = launch_cfg<T, AKS, BKS, 2, 4, 8, 5>(p, st);
-  else rc = launch_cfg<T, AKS, BKS, 2, 2, 4, 4>(p, st);
+  else if (plan.cfg == 2) rc = launch_cfg<T, AKS, BKS, 2, 2, 4, 4>(p, st);
+  else rc = launch_cfg<T, AKS, BKS, 2, 2, 2, 2>(p, st);
   if (rc || plan.splits == 1) return rc;
   hipLaunchKernelGGL((join_kernel<T>), dim3(grid_of((long)p.M * ((p.N + 7) / 8))), dim3(256), 0, st, (const float*)part, p.e, (long)p.M, p.N, plan.splits);
   HI3D_LAUNCH_CHECK();
