@@ -251,18 +251,16 @@ struct Frags {
 // WM x WN waves, each 16 MT x 16 NT of the output; two tiles of the contraction in LDS, the next one on its way while one is used.
 // The weight-side fragment is the first operand of the matrix instruction, so that a lane holds 4 consecutive columns of one output row.
 template <typename T, bool AKS, bool BKS, int WM, int WN, int MT, int NT>
-__global__ __launch_bounds__(WM * WN * 64, MT == 2 ? 4 : 2) void mat_kernel(const MatParams p) {
+__device__ __forceinline__ void mat_tile(const MatParams& p, int bid, char* smem) {
 #if __HIP_DEVICE_COMPILE__
   constexpr int NW = WM * WN, BM = 16 * MT * WM, BN = 16 * NT * WN;
   constexpr int ABYTES = BM * 128, STAGE = (BM + BN) * 128;
-  extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = w / WN, wn = w % WN;
 
   // block -> tile: neighbours in the order go to one XCD (its L2 keeps what they share); `group` m-tiles are walked for each n-tile
   const int nblk = p.nbm * p.nbn;
-  int bid = blockIdx.x;
   const int ks = bid / nblk;
   bid -= ks * nblk;
   const int q = nblk >> 3, r = nblk & 7, xcd = bid & 7, idx = bid >> 3;
@@ -501,6 +499,19 @@ __global__ __launch_bounds__(WM * WN * 64, MT == 2 ? 4 : 2) void mat_kernel(cons
 #endif
 }
 
+template <typename T, bool AKS, bool BKS, int WM, int WN, int MT, int NT>
+__global__ __launch_bounds__(WM * WN * 64, MT == 2 ? 4 : 2) void mat_kernel(const MatParams p) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  mat_tile<T, AKS, BKS, WM, WN, MT, NT>(p, blockIdx.x, smem);
+}
+// dw and dx of a layer in one launch, where neither fills the chip by itself: the first `first` blocks are dw's (the longer ones)
+template <typename T, int WM, int WN, int MT, int NT>
+__global__ __launch_bounds__(WM * WN * 64, MT == 2 ? 4 : 2) void both_gradients_kernel(const MatParams dw, const MatParams dx, int first) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  if ((int)blockIdx.x < first) mat_tile<T, true, true, WM, WN, MT, NT>(dw, blockIdx.x, smem);
+  else mat_tile<T, false, true, WM, WN, MT, NT>(dx, blockIdx.x - first, smem);
+}
+
 // ---- few rows ---------------------------------------------------------------------------------------------------------------------
 // y for at most 16 MT rows of x: the weights are all there is to read, once.  A block takes 16 / CS columns of the output and its 16 waves a
 // 16th of the contraction each, straight from memory into matrix operands -- no LDS, no padded copies: any pitch and alignment -- with U
@@ -597,31 +608,22 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, Epilogue e
   }
 }
 
-// rows of any pitch and alignment -> rows padded with zeros to a multiple of 8 elements, 16-byte aligned
-template <typename T>
-__global__ __launch_bounds__(256) void pad_kernel(const T* in, T* out, long rows, int cols, long ld) {
-  const int cpr = (cols + 7) / 8;
-  for (long c = (long)blockIdx.x * 256 + threadIdx.x; c < rows * cpr; c += (long)gridDim.x * 256) {
-    const long r = c / cpr;
-    const int e = (int)(c - r * cpr) * 8;
-    Pack<T, 8> k;
-    fetch(in + r * ld + e, cols - e, e, k);
-    *(Pack<T, 8>*)(out + r * (long)cpr * 8 + e) = k;
-  }
-}
-
-// dz = dy act'(z), rounded to the operands' type for the matrix instruction (its sums stay fp32), rows padded as above; and the column
-// sums of the unrounded dz, one row of partial sums per block row.  256 columns x 8 row lanes a block.
+// What the products need first, in one launch:
+//   dz = dy act'(z), rounded to the operands' type for the matrix instruction (its sums stay fp32), in rows padded with zeros to a multiple of 8
+//   elements; and the column sums of the unrounded dz, one row of partial sums per block row (256 columns x 8 row lanes a block);
+//   up to two operands whose rows cannot be read in place, padded likewise.
 struct SlopeParams {
   const void* dy; const void* z; void* dz; float* part;
   long M, lddy, ldz;
   int N, act, rows;                        // rows: of a block
 };
+struct PadParams { const void* in; void* out; long rows, ld; int cols, blocks; };
+
 template <typename T>
-__global__ __launch_bounds__(256) void slope_kernel(const SlopeParams p) {
+__device__ __forceinline__ void slope(const SlopeParams& p, int bx, int by) {
   __shared__ float lds[8][256];
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, c = blockIdx.x * 256 + tx * 8, n = p.N - c;
-  const long r0 = (long)blockIdx.y * p.rows, r1 = min(p.M, r0 + p.rows);
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, c = bx * 256 + tx * 8, n = p.N - c;
+  const long r0 = (long)by * p.rows, r1 = min(p.M, r0 + p.rows);
   const long ldo = (p.N + 7) / 8 * 8;
   float s[8] = {};
   if (n > 0)
@@ -647,13 +649,31 @@ __global__ __launch_bounds__(256) void slope_kernel(const SlopeParams p) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) lds[ty][tx * 8 + j] = s[j];
   __syncthreads();
-  const int col = blockIdx.x * 256 + threadIdx.x;
+  const int col = bx * 256 + threadIdx.x;
   if (col < p.N) {
     float t = 0.0f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) t += lds[k][threadIdx.x];
-    p.part[(long)blockIdx.y * p.N + col] = t;
+    p.part[(long)by * p.N + col] = t;
   }
+}
+template <typename T>
+__device__ __forceinline__ void pad_rows(const PadParams& p, int block) {
+  const int cpr = (p.cols + 7) / 8;
+  for (long c = (long)block * 256 + threadIdx.x; c < p.rows * cpr; c += (long)p.blocks * 256) {
+    const long r = c / cpr;
+    const int e = (int)(c - r * cpr) * 8;
+    Pack<T, 8> k;
+    fetch((const T*)p.in + r * p.ld + e, p.cols - e, e, k);
+    *(Pack<T, 8>*)((T*)p.out + r * (long)cpr * 8 + e) = k;
+  }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void prepare_kernel(const SlopeParams s, int across, int slope_blocks, const PadParams a, const PadParams b) {
+  const int bid = blockIdx.x;
+  if (bid < slope_blocks) slope<T>(s, bid % across, bid / across);
+  else if (bid < slope_blocks + a.blocks) pad_rows<T>(a, bid - slope_blocks);
+  else pad_rows<T>(b, bid - slope_blocks - a.blocks);
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------------
@@ -686,6 +706,29 @@ Plan plan_of(long M, long N, long K) {
   return best;
 }
 
+// dx (M x K over N) and dw (N x K over M) in one launch of the same small tile, where that is estimated to be faster than one after the other
+struct BothPlan { bool use; Plan dx, dw; };
+BothPlan both_plan_of(long M, long N, long K, const Plan& dx, const Plan& dw) {
+  BothPlan best = {false, dx, dw};
+  double least = dx.us + dw.us + 3.0;                    // (a launch between them)
+  const long xs = (N + BK - 1) / BK, ws = (M + BK - 1) / BK;
+  for (int c = 2; c < 4; ++c) {
+    const Config& f = CONFIGS[c];
+    const long tx = ((M + f.bm - 1) / f.bm) * ((K + f.bn - 1) / f.bn), tw = ((N + f.bm - 1) / f.bm) * ((K + f.bn - 1) / f.bn), slots = (long)f.per_cu * CUS;
+    for (long s = 1; s <= MAX_SPLITS && s <= ws; ++s) {
+      const long per = (ws + s - 1) / s;
+      if ((ws + per - 1) / per != s) continue;
+      const long blocks = tx + tw * s;
+      if (s > 1 && blocks > 4 * slots) break;
+      const double on_cu = blocks >= slots ? f.per_cu : blocks > CUS ? (double)blocks / CUS : 1.0, step = f.one + (f.full - f.one) * (on_cu - 1.0) / (f.per_cu - 1);
+      const double x = xs * step + f.fixed, w = per * step + f.fixed, all = (tx * x + tw * s * w) / (on_cu * CUS);
+      const double us = (all > w ? (all > x ? all : x) : (w > x ? w : x)) + 0.5 * (x < w ? x : w) * (blocks > slots) + (s > 1 ? 4.5 + (double)N * K * (8.0 * s + 2.0) / 6.0e6 : 0.0);
+      if (us < least) { least = us; best = {true, {c, 1, (int)xs, us}, {c, (int)s, (int)per, us}}; }
+    }
+  }
+  return best;
+}
+
 long round256(long b) { return (b + 255) & ~255L; }
 long part_bytes(const Plan& p, long M, long N) { return p.splits > 1 ? round256(p.splits * M * N * 4) : 0; }
 
@@ -700,19 +743,36 @@ int launch_cfg(const MatParams& p, hipStream_t st) {
 }
 unsigned grid_of(long items) { const long n = (items + 255) / 256; return (unsigned)(n < 1 ? 1 : n > 8192 ? 8192 : n); }
 
+void set_plan(MatParams* p, const Plan& plan, float* part) {
+  const Config& f = CONFIGS[plan.cfg];
+  p->nbm = (p->M + f.bm - 1) / f.bm; p->nbn = (p->N + f.bn - 1) / f.bn;
+  p->splits = plan.splits; p->per = plan.per; p->part = plan.splits > 1 ? part : nullptr;
+  p->group = 8;
+}
+template <typename T>
+int join(const MatParams& p, hipStream_t st) {
+  if (p.splits == 1) return 0;
+  hipLaunchKernelGGL((join_kernel<T>), dim3(grid_of((long)p.M * ((p.N + 7) / 8))), dim3(256), 0, st, (const float*)p.part, p.e, (long)p.M, p.N, p.splits);
+  HI3D_LAUNCH_CHECK();
+  return 0;
+}
 template <typename T, bool AKS, bool BKS>
 int launch_mat(MatParams p, const Plan& plan, float* part, hipStream_t st) {
-  const Config& f = CONFIGS[plan.cfg];
-  p.nbm = (p.M + f.bm - 1) / f.bm; p.nbn = (p.N + f.bn - 1) / f.bn;
-  p.splits = plan.splits; p.per = plan.per; p.part = plan.splits > 1 ? part : nullptr;
-  p.group = 8;
+  set_plan(&p, plan, part);
   int rc;
   if (plan.cfg == 0) rc = launch_cfg<T, AKS, BKS, 2, 4, 8, 4>(p, st);
   else if (plan.cfg == 1) rc = launch_cfg<T, AKS, BKS, 2, 4, 8, 5>(p, st);
   else if (plan.cfg == 2) rc = launch_cfg<T, AKS, BKS, 2, 2, 4, 4>(p, st);
   else rc = launch_cfg<T, AKS, BKS, 2, 2, 2, 2>(p, st);
-  if (rc || plan.splits == 1) return rc;
-  hipLaunchKernelGGL((join_kernel<T>), dim3(grid_of((long)p.M * ((p.N + 7) / 8))), dim3(256), 0, st, (const float*)part, p.e, (long)p.M, p.N, plan.splits);
+  return rc ? rc : join<T>(p, st);
+}
+template <typename T, int WM, int WN, int MT, int NT>
+int launch_both(const MatParams& dw, const MatParams& dx, hipStream_t st) {
+  constexpr int LDS = 2 * (16 * MT * WM + 16 * NT * WN) * 128 + 16 * NT * WN * 4;
+  static bool done[HI3D_MAX_DEVICES];
+  if (const int rc = hi3d_raise_lds_limit((const void*)both_gradients_kernel<T, WM, WN, MT, NT>, LDS, done)) return rc;
+  const int first = dw.nbm * dw.nbn * dw.splits;
+  hipLaunchKernelGGL((both_gradients_kernel<T, WM, WN, MT, NT>), dim3((unsigned)(first + dx.nbm * dx.nbn * dx.splits)), dim3(WM * WN * 64), LDS, st, dw, dx, first);
   HI3D_LAUNCH_CHECK();
   return 0;
 }
@@ -721,22 +781,23 @@ int launch_mat(MatParams p, const Plan& plan, float* part, hipStream_t st) {
 bool in_place(const void* p, long ld, long cols) { return !((uintptr_t)p & 15) && ld % 8 == 0 && cols % 8 == 0; }
 long padded_bytes(long rows, long cols) { return round256(rows * ((cols + 7) / 8 * 8) * 2); }
 
-template <typename T>
-int pad(const void* in, void* out, long rows, int cols, long ld, hipStream_t st) {
-  hipLaunchKernelGGL((pad_kernel<T>), dim3(grid_of(rows * ((cols + 7) / 8))), dim3(256), 0, st, (const T*)in, (T*)out, rows, cols, ld);
-  HI3D_LAUNCH_CHECK();
-  return 0;
-}
-
 struct Operand { const void* p; long ld; };
-// the operand itself, or -- where the kernel cannot read it in place -- a padded copy at *ws, which moves on
-template <typename T>
-int place(const void* p, long rows, int cols, long ld, char** ws, Operand* o, hipStream_t st) {
-  if (in_place(p, ld, cols)) { *o = {p, ld}; return 0; }
+// the operand itself, or -- where the kernel cannot read it in place -- where its padded copy will be at *ws, which moves on; the copy is `job`'s
+Operand place(const void* p, long rows, int cols, long ld, char** ws, PadParams* job) {
+  if (in_place(p, ld, cols)) return {p, ld};
   char* const to = *ws;
   *ws += padded_bytes(rows, cols);
-  *o = {to, (cols + 7L) / 8 * 8};
-  return pad<T>(p, to, rows, cols, ld, st);
+  const long blocks = (rows * ((cols + 7L) / 8) + 1023) / 1024;
+  *job = {p, to, rows, ld, cols, (int)(blocks < 4096 ? blocks : 4096)};
+  return {to, (cols + 7L) / 8 * 8};
+}
+template <typename T>
+int prepare(const SlopeParams& s, int slices, const PadParams& a, const PadParams& b, hipStream_t st) {
+  const int across = (s.N + 255) / 256, n = across * slices;
+  if (n + a.blocks + b.blocks == 0) return 0;
+  hipLaunchKernelGGL((prepare_kernel<T>), dim3((unsigned)(n + a.blocks + b.blocks)), dim3(256), 0, st, s, across > 0 ? across : 1, n, a, b);
+  HI3D_LAUNCH_CHECK();
+  return 0;
 }
 
 constexpr int SLOPE_BLOCKS = 2048;
@@ -782,16 +843,25 @@ int few_rows(const FewParams& p, hipStream_t st) {
   return launch_few<T, 1, 1>(p, st);
 }
 
-struct FwdNeeds { long x, w, part; Plan plan; };
+// The rows that tiles take: all of them, or -- where up to 32 rows behind the last whole 256 would cost more as tiles than as streamed
+// weights -- all but those (4112 rows of 1280 -> 5120: 4096 fill the chip once, with the 16 in tiles of 128 it takes 75 us, with them streamed 66, gelu and z kept).
+struct FwdNeeds { long rows, x, w, part; Plan plan; };
 FwdNeeds fwd_needs(const hi3d_linear_desc* d) {
-  if (d->M <= FEW) return {};
-  FwdNeeds n = {0, 0, 0, plan_of(d->M, d->N, d->K)};
-  if (!in_place(d->x, d->ldx, d->K)) n.x = padded_bytes(d->M, d->K);
+  FwdNeeds n = {};
+  if (d->M <= FEW) return n;
+  n.rows = d->M;
+  n.plan = plan_of(d->M, d->N, d->K);
+  const long rest = d->M % 256;
+  if (d->M > 256 && rest && rest <= FEW) {
+    const Plan p = plan_of(d->M - rest, d->N, d->K);
+    if (p.us + 4.0 + (double)d->N * d->K * 2.0 / 2.5e6 < n.plan.us) { n.rows = d->M - rest; n.plan = p; }
+  }
+  if (!in_place(d->x, d->ldx, d->K)) n.x = padded_bytes(n.rows, d->K);
   if (!in_place(d->w, d->ldw, d->K)) n.w = padded_bytes(d->N, d->K);
-  n.part = part_bytes(n.plan, d->M, d->N);
+  n.part = part_bytes(n.plan, n.rows, d->N);
   return n;
 }
-struct BwdNeeds { long dz, x, w, part, cols; Plan dx, dw; };
+struct BwdNeeds { long dz, x, w, part, cols; Plan dx, dw; bool both; };
 BwdNeeds bwd_needs(const hi3d_linear_desc* d) {
   BwdNeeds n = {};
   const bool copy = d->act != HI3D_ACT_NONE || !in_place(d->dy, d->lddy, d->N);
@@ -800,6 +870,10 @@ BwdNeeds bwd_needs(const hi3d_linear_desc* d) {
   if (d->dx && !in_place(d->w, d->ldw, d->K)) n.w = padded_bytes(d->N, d->K);
   n.dx = plan_of(d->M, d->K, d->N);
   n.dw = plan_of(d->N, d->K, d->M);
+  if (d->dx && d->dw) {
+    const BothPlan b = both_plan_of(d->M, d->N, d->K, n.dx, n.dw);
+    n.both = b.use; n.dx = b.dx; n.dw = b.dw;
+  }
   const long a = d->dx ? part_bytes(n.dx, d->M, d->K) : 0, b = d->dw ? part_bytes(n.dw, d->N, d->K) : 0;
   n.part = a > b ? a : b;
   if (d->db) n.cols = round256((long)slope_slices(d->M, d->N) * d->N * 4);
@@ -808,19 +882,23 @@ BwdNeeds bwd_needs(const hi3d_linear_desc* d) {
 
 template <typename T>
 int fwd(const hi3d_linear_desc* d, hipStream_t st) {
-  const Epilogue e = {d->bias, d->residual, d->y, d->z, (long)d->ldr, (long)d->N, d->bias_dtype, d->act};
-  if (d->M <= FEW) {
-    const FewParams p = {d->x, d->w, e, (long)d->ldx, (long)d->ldw, (int)d->M, d->N, d->K};
-    return few_rows<T>(p, st);
-  }
   const FwdNeeds n = fwd_needs(d);
+  const Epilogue e = {d->bias, d->residual, d->y, d->z, (long)d->ldr, (long)d->N, d->bias_dtype, d->act};
+  if (n.rows < d->M) {
+    const long r = n.rows;
+    auto down = [&](const void* p, long ld) { return p ? (void*)((T*)p + r * ld) : nullptr; };
+    const Epilogue f = {d->bias, down(d->residual, d->ldr), down(d->y, d->N), down(d->z, d->N), (long)d->ldr, (long)d->N, d->bias_dtype, d->act};
+    const FewParams p = {down(d->x, d->ldx), d->w, f, (long)d->ldx, (long)d->ldw, (int)(d->M - r), d->N, d->K};
+    const int rc = few_rows<T>(p, st);
+    if (rc || !r) return rc;
+  }
   char* ws = (char*)d->ws;
-  Operand x, w;
-  if (const int rc = place<T>(d->x, d->M, d->K, d->ldx, &ws, &x, st)) return rc;
-  if (const int rc = place<T>(d->w, d->N, d->K, d->ldw, &ws, &w, st)) return rc;
+  PadParams jx = {}, jw = {};
+  const Operand x = place(d->x, n.rows, d->K, d->ldx, &ws, &jx), w = place(d->w, d->N, d->K, d->ldw, &ws, &jw);
+  if (const int rc = prepare<T>(SlopeParams{}, 0, jx, jw, st)) return rc;
   MatParams p = {};
   p.A = (const char*)x.p; p.B = (const char*)w.p; p.lda = x.ld; p.ldb = w.ld;
-  p.M = (int)d->M; p.N = d->N; p.K = d->K;
+  p.M = (int)n.rows; p.N = d->N; p.K = d->K;
   p.e = e;
   return launch_mat<T, false, false>(p, n.plan, (float*)ws, st);
 }
@@ -830,37 +908,34 @@ int bwd(const hi3d_linear_desc* d, hipStream_t st) {
   const BwdNeeds n = bwd_needs(d);
   char* ws = (char*)d->ws;
   Operand dz = {d->dy, (long)d->lddy};
-  void* to = nullptr;
-  if (n.dz) { to = ws; dz = {ws, (d->N + 7L) / 8 * 8}; ws += n.dz; }
-  if (n.dz || d->db) {
-    float* const cols = d->db ? (float*)ws : nullptr;
-    const int rows = slope_rows(d->M, d->N), slices = slope_slices(d->M, d->N);
-    const SlopeParams p = {d->dy, d->z, to, cols, (long)d->M, (long)d->lddy, (long)d->ldz, d->N, d->act, rows};
-    hipLaunchKernelGGL((slope_kernel<T>), dim3((d->N + 255) / 256, slices), dim3(256), 0, st, p);
-    HI3D_LAUNCH_CHECK();
-    if (d->db)
-      if (const int rc = hi3d_column_reduce(cols, d->db, nullptr, d->bias_dtype, 0, slices, d->N, d->N, st)) return rc;
-    ws += n.cols;
+  SlopeParams sp = {d->dy, d->z, nullptr, nullptr, (long)d->M, (long)d->lddy, (long)d->ldz, d->N, d->act, slope_rows(d->M, d->N)};
+  if (n.dz) { sp.dz = ws; dz = {ws, (d->N + 7L) / 8 * 8}; ws += n.dz; }
+  if (d->db) { sp.part = (float*)ws; ws += n.cols; }
+  const int slices = (n.dz || d->db) ? slope_slices(d->M, d->N) : 0;
+  PadParams jw = {}, jx = {};
+  Operand w = {}, x = {};
+  if (d->dx) w = place(d->w, d->N, d->K, d->ldw, &ws, &jw);
+  if (d->dw) x = place(d->x, d->M, d->K, d->ldx, &ws, &jx);
+  if (const int rc = prepare<T>(sp, slices, jw, jx, st)) return rc;
+  if (d->db)
+    if (const int rc = hi3d_column_reduce(sp.part, d->db, nullptr, d->bias_dtype, 0, slices, d->N, d->N, st)) return rc;
+  float* const part = (float*)ws;                   // (dx's and dw's in turn: they follow each other on the stream, and in one launch only dw is split)
+  MatParams px = {}, pw = {};
+  px.A = (const char*)dz.p; px.B = (const char*)w.p; px.lda = dz.ld; px.ldb = w.ld;
+  px.M = (int)d->M; px.N = d->K; px.K = d->N;
+  px.e = {nullptr, nullptr, d->dx, nullptr, 0, (long)d->K, HI3D_F32, HI3D_ACT_NONE};
+  pw.A = (const char*)dz.p; pw.B = (const char*)x.p; pw.lda = dz.ld; pw.ldb = x.ld;
+  pw.M = d->N; pw.N = d->K; pw.K = (int)d->M;
+  pw.e = {nullptr, nullptr, d->dw, nullptr, 0, (long)d->K, HI3D_F32, HI3D_ACT_NONE};
+  if (n.both) {
+    set_plan(&px, n.dx, part);
+    set_plan(&pw, n.dw, part);
+    const int rc = n.dx.cfg == 2 ? launch_both<T, 2, 2, 4, 4>(pw, px, st) : launch_both<T, 2, 2, 2, 2>(pw, px, st);
+    return rc ? rc : join<T>(pw, st);
   }
-  if (d->dx) {
-    Operand w;
-    if (const int rc = place<T>(d->w, d->N, d->K, d->ldw, &ws, &w, st)) return rc;
-    MatParams p = {};
-    p.A = (const char*)dz.p; p.B = (const char*)w.p; p.lda = dz.ld; p.ldb = w.ld;
-    p.M = (int)d->M; p.N = d->K; p.K = d->N;
-    p.e = {nullptr, nullptr, d->dx, nullptr, 0, (long)d->K, HI3D_F32, HI3D_ACT_NONE};
-    if (const int rc = launch_mat<T, false, true>(p, n.dx, (float*)((char*)d->ws + n.dz + n.cols + n.w + n.x), st)) return rc;
-  }
-  if (d->dw) {
-    Operand x;
-    if (const int rc = place<T>(d->x, d->M, d->K, d->ldx, &ws, &x, st)) return rc;
-    MatParams p = {};
-    p.A = (const char*)dz.p; p.B = (const char*)x.p; p.lda = dz.ld; p.ldb = x.ld;
-    p.M = d->N; p.N = d->K; p.K = (int)d->M;
-    p.e = {nullptr, nullptr, d->dw, nullptr, 0, (long)d->K, HI3D_F32, HI3D_ACT_NONE};
-    if (const int rc = launch_mat<T, true, true>(p, n.dw, (float*)((char*)d->ws + n.dz + n.cols + n.w + n.x), st)) return rc;
-  }
-  return 0;
+  if (d->dx)
+    if (const int rc = launch_mat<T, false, true>(px, n.dx, part, st)) return rc;
+  return d->dw ? launch_mat<T, true, true>(pw, n.dw, part, st) : 0;
 }
 
 }  // namespace

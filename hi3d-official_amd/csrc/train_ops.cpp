@@ -220,6 +220,32 @@ const float* scalar_of(const OptTensor& t, const Tensor& on, const char* what) {
   return t->data_ptr<float>();
 }
 
+using Spans = std::vector<std::pair<uintptr_t, uintptr_t>>;
+void span_of(const Tensor& t, Spans& to) {
+  const uintptr_t b = (uintptr_t)t.data_ptr();
+  if (const int64_t n = t.numel()) to.emplace_back(b, b + n * t.element_size());
+}
+// whether what is written overlaps nothing else (lists of views into one buffer, or of tensors in the order of their allocation, are in order
+// already and merged in linear time)
+bool apart(Spans (&written)[4], Spans& read) {
+  Spans all;
+  for (Spans& l : written) {
+    if (!std::is_sorted(l.begin(), l.end())) std::sort(l.begin(), l.end());
+    Spans both(all.size() + l.size());
+    std::merge(all.begin(), all.end(), l.begin(), l.end(), both.begin());
+    all.swap(both);
+  }
+  for (size_t i = 1; i < all.size(); ++i)
+    if (all[i].first < all[i - 1].second) return false;
+  if (!std::is_sorted(read.begin(), read.end())) std::sort(read.begin(), read.end());
+  size_t i = 0;
+  for (const auto& r : read) {
+    while (i < all.size() && all[i].second <= r.first) ++i;
+    if (i < all.size() && all[i].first < r.second) return false;
+  }
+  return true;
+}
+
 void adamw_(at::TensorList params, at::TensorList grads, at::TensorList exp_avg, at::TensorList exp_avg_sq, at::TensorList copies, double lr, double beta1,
             double beta2, double eps, double weight_decay, int64_t step, const OptTensor& step_t, const OptTensor& lr_t, const OptTensor& grad_scale,
             const OptTensor& found_inf) {
@@ -236,12 +262,9 @@ void adamw_(at::TensorList params, at::TensorList grads, at::TensorList exp_avg,
   // one launch per combination of types; the tensors of a combination keep their order
   struct Kind { int p, g, c; std::vector<hi3d_adamw_tensor> t; };
   std::vector<Kind> kinds;
-  std::vector<std::pair<uintptr_t, uintptr_t>> written;
-  written.reserve(4 * n);
-  auto writes = [&](const Tensor& t) {
-    const uintptr_t b = (uintptr_t)t.data_ptr();
-    if (t.numel()) written.emplace_back(b, b + t.numel() * t.element_size());
-  };
+  Spans written[4], read;                     // parameters, both moments, copies; gradients
+  for (Spans& l : written) l.reserve(n);
+  read.reserve(n);
   for (size_t i = 0; i < n; ++i) {
     const Tensor &p = params[i], &g = grads[i], &m = exp_avg[i], &v = exp_avg_sq[i];
     want_gpu(p, on, name);
@@ -254,7 +277,7 @@ void adamw_(at::TensorList params, at::TensorList grads, at::TensorList exp_avg,
     TORCH_CHECK(m.scalar_type() == at::kFloat && v.scalar_type() == at::kFloat, name, ": tensor ", i, ": moments must be fp32");
     hi3d_adamw_tensor d = {p.data_ptr(), g.data_ptr(), m.data_ptr<float>(), v.data_ptr<float>(), nullptr, p.numel()};
     int cd = HI3D_BF16;
-    writes(p); writes(m); writes(v);
+    span_of(p, written[0]); span_of(m, written[1]); span_of(v, written[2]); span_of(g, read);
     if (!copies.empty()) {
       const Tensor& c = copies[i];
       want_gpu(c, on, name);
@@ -263,21 +286,13 @@ void adamw_(at::TensorList params, at::TensorList grads, at::TensorList exp_avg,
       TORCH_CHECK(c.sizes() == p.sizes() && c.strides() == p.strides(), name, ": tensor ", i, ": the working copy must have the parameter's shape and strides");
       cd = dtype_of(c, name);
       d.copy = c.data_ptr();
-      writes(c);
+      span_of(c, written[3]);
     }
     auto k = std::find_if(kinds.begin(), kinds.end(), [&](const Kind& q) { return q.p == pd && q.g == gd && q.c == cd; });
     if (k == kinds.end()) { kinds.push_back({pd, gd, cd, {}}); k = kinds.end() - 1; k->t.reserve(n); }
     k->t.push_back(d);
   }
-  std::sort(written.begin(), written.end());
-  for (size_t i = 1; i < written.size(); ++i)
-    TORCH_CHECK(written[i].first >= written[i - 1].second, name, ": tensors that are written share memory (the same parameter twice?)");
-  for (size_t i = 0; i < n; ++i) {             // a gradient that another block's update overwrites
-    if (!grads[i].numel()) continue;
-    const uintptr_t b = (uintptr_t)grads[i].data_ptr(), e = b + grads[i].numel() * grads[i].element_size();
-    auto it = std::lower_bound(written.begin(), written.end(), std::make_pair(b, (uintptr_t)0));
-    TORCH_CHECK((it == written.end() || it->first >= e) && (it == written.begin() || (it - 1)->second <= b), name, ": a gradient shares memory with a tensor that is written");
-  }
+  TORCH_CHECK(apart(written, read), name, ": a tensor that is written shares memory with another of the call (the same parameter twice?)");
   const Guard guard(on.device());
   hi3d_adamw_coefs_t c = {};
   c.beta1 = (float)beta1; c.one_minus_beta1 = (float)(1.0 - beta1); c.beta2 = (float)beta2; c.one_minus_beta2 = (float)(1.0 - beta2); c.eps = (float)eps;
