@@ -17,6 +17,8 @@ typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(8))) __bf16 bfx8;
 
 constexpr int BK = 64;
+// elements between rows that a tile's 32-bit offsets reach (320 rows of 2 bytes an element, 256 rows of 4): more is copied, or stored without them
+constexpr long MOST_PITCH = 0x200000, MOST_WIDTH = 0x100000;
 
 // ---- activations ------------------------------------------------------------------------------------------------------------------
 // Phi(-a) = exp(-a^2 / 2) P(t), t = 1 / (1 + 0.3 a), a >= 0: P of degree 8 without constant term, fitted to the Mills ratio over
@@ -369,7 +371,7 @@ __device__ __forceinline__ void mat_tile(const MatParams& p, int bid, char* smem
   constexpr unsigned NONE = 0x80000000u;
   const int fr = lane & 15, fg = lane >> 4;
   const int cols = p.N - n0;                        // of the tile that exist
-  const bool fits = p.N % 8 == 0 && (!p.e.res || (p.e.ldr % 8 == 0 && ((unsigned long)p.e.res & 15) == 0));      // 16-byte accesses do
+  const bool fits = p.N % 8 == 0 && (!p.e.res || (p.e.ldr % 8 == 0 && p.e.ldr <= MOST_PITCH && ((unsigned long)p.e.res & 15) == 0));      // 16-byte accesses do
   const bool wide = p.part || p.e.res || !fits;     // fp32 through LDS
   const int wrow = wm * 16 + fr, wcol = wn * 16 * NT + fg * 4;
   f32x4 bias[NT];
@@ -385,8 +387,8 @@ __device__ __forceinline__ void mat_tile(const MatParams& p, int bid, char* smem
     const bool in = c < SROWS * CPR && q * 8 < cols;
     hat[t] = in ? r * HROW + q * 16 : 0;
     fat[t] = in ? r * FROW + q * 16 : 0;
-    off[t] = in ? (unsigned)((row * (int)ldo + q * 8) * esz) : NONE;
-    roff[t] = in ? (unsigned)((row * (int)p.e.ldr + q * 8) * 2) : NONE;
+    off[t] = in ? ((unsigned)row * (unsigned)ldo + q * 8) * esz : NONE;
+    roff[t] = in ? ((unsigned)row * (unsigned)p.e.ldr + q * 8) * 2 : NONE;
   }
   auto window = [&](const void* base, long ld, int size, int i) {        // rows m0 + 16 i ... of a matrix of M rows, from column n0
     const long rows = p.M - m0 - 16 * i, valid = rows > 0 ? ((rows - 1) * ld + cols) * size : 0;
@@ -778,7 +780,7 @@ int launch_both(const MatParams& dw, const MatParams& dx, hipStream_t st) {
 }
 
 // whether rows of `cols` elements can be read in place
-bool in_place(const void* p, long ld, long cols) { return !((uintptr_t)p & 15) && ld % 8 == 0 && cols % 8 == 0; }
+bool in_place(const void* p, long ld, long cols) { return !((uintptr_t)p & 15) && ld % 8 == 0 && ld <= MOST_PITCH && cols % 8 == 0; }
 long padded_bytes(long rows, long cols) { return round256(rows * ((cols + 7) / 8 * 8) * 2); }
 
 struct Operand { const void* p; long ld; };
@@ -817,12 +819,7 @@ const char* bad_desc(const hi3d_linear_desc* d) {
   if (d->act < HI3D_ACT_NONE || d->act > HI3D_ACT_RELU) return "linear training: unknown activation";
   return nullptr;
 }
-// tiles address their rows in 32 bits: 320 rows of 2 bytes an element
-bool too_big(const hi3d_linear_desc* d) {
-  const long most = 0x7ffffff0L / 640;
-  return d->M > 0x7fff0000L || d->N > most || d->K > most || d->N > 0x100000 || d->K > 0x100000 ||
-         (d->M > 1 && (d->ldx > most || d->lddy > most || d->ldz > (1L << 40) || d->ldr > (1L << 40))) || (d->N > 1 && d->ldw > most);
-}
+bool too_big(const hi3d_linear_desc* d) { return d->M > 0x7fff0000L || d->N > MOST_WIDTH || d->K > MOST_WIDTH; }
 
 // Up to 32 rows the weights are streamed by few_rows_kernel, above that the tiles are faster (N = K = 4096, 32 / 48 / 65 rows: streamed 14 /
 // 19 us, tiles 18 us for up to 128).
@@ -948,7 +945,7 @@ extern "C" int64_t hi3d_linear_fwd_workspace_bytes(const hi3d_linear_desc* d) {
 
 extern "C" int hi3d_linear_fwd(const hi3d_linear_desc* d, void* stream) {
   if (const char* why = bad_desc(d)) HI3D_FAIL(HI3D_EINVAL, why);
-  if (too_big(d)) HI3D_FAIL(HI3D_ESHAPE, "linear_fwd: a size or pitch is over what a tile addresses");
+  if (too_big(d)) HI3D_FAIL(HI3D_ESHAPE, "linear_fwd: a width is over 1048576, or too many rows");
   if (d->M == 0) return 0;
   if (!d->x || !d->w || !d->y) HI3D_FAIL(HI3D_EINVAL, "linear_fwd: null pointer");
   if ((d->M > 1 && (d->ldx < d->K || (d->residual && d->ldr < d->N))) || (d->N > 1 && d->ldw < d->K)) HI3D_FAIL(HI3D_EINVAL, "linear_fwd: row pitch below the width");
@@ -965,7 +962,7 @@ extern "C" int64_t hi3d_linear_bwd_workspace_bytes(const hi3d_linear_desc* d) {
 
 extern "C" int hi3d_linear_bwd(const hi3d_linear_desc* d, void* stream) {
   if (const char* why = bad_desc(d)) HI3D_FAIL(HI3D_EINVAL, why);
-  if (too_big(d)) HI3D_FAIL(HI3D_ESHAPE, "linear_bwd: a size or pitch is over what a tile addresses");
+  if (too_big(d)) HI3D_FAIL(HI3D_ESHAPE, "linear_bwd: a width is over 1048576, or too many rows");
   const hipStream_t st = (hipStream_t)stream;
   if (d->M == 0) {                       // sums over no rows
     if (d->db)

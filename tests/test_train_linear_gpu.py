@@ -180,6 +180,25 @@ def test_what_lies_around_the_operands_is_not_read_into_results(dev, ns):
         assert all(torch.equal(p, q) for p, q in zip(e, f))
 
 
+def test_rows_far_apart(dev, ns):
+    """Pitches that a tile's 32-bit offsets do not reach, for every operand."""
+    M, N, K, ld = 65, 72, 96, 3_000_000
+    c = [rnd((M, K), 1, "bf16"), rnd((N, K), 2, "bf16"), rnd((M, N), 3, "bf16"), rnd((M, N), 4, "bf16"), rnd((M, N), 5, "bf16")]
+    flat = torch.zeros((N - 1) * ld + N * 5 + K, dtype=torch.bfloat16, device=dev)
+    far, at = [], 0
+    for t in c:                                    # all in one buffer, side by side
+        v = flat.as_strided(t.shape, (ld, 1), at)
+        v.copy_(t)
+        far.append(v)
+        at += (t.shape[1] + 7) // 8 * 8
+    b = rnd((N,), 6).to(dev)
+    c = [t.to(dev) for t in c]
+
+    def run(x, w, r, dy, z):
+        return ns.linear_act(x, w, b, r, "gelu", True) + ns.linear_act_bwd(dy, x, w, z, b, "gelu", True, True) + ns.linear_act_bwd(dy, x, w, None, b, "none", True, True)
+    assert all(torch.equal(p, q) for p, q in zip(run(*far), run(*c)))
+
+
 def test_no_rows(dev, ns):
     x, w, b = torch.zeros(0, 40, device=dev).bfloat16(), rnd((24, 40), 1, "bf16").to(dev), rnd((24,), 2).to(dev)
     y, z = ns.linear_act(x, w, b, x.new_zeros(0, 24), "gelu", True)
