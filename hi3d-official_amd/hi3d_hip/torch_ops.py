@@ -7,6 +7,7 @@ that a module written against torch tensors reaches the gfx950 kernels as
     torch.ops.hi3d.attn_d64(q, k, v, B, H, S_q, S_kv, scale)
     torch.ops.hi3d.attn_temporal(qkv, B, T, S, H, scale)    # VideoTransformerBlock's attention over frames
     torch.ops.hi3d.groupnorm_silu / layernorm / linear / conv3x3 / ffn_geglu
+    torch.ops.hi3d.layernorm_fwd / add_layernorm_fwd / layernorm_bwd / linear_act / linear_act_bwd / adamw_     # training (csrc/train_ops.cpp; autograd: train.py)
 
 which is the binding INTEGRATION.md (B) shows for the reference's ATTENTION_MODES plug-in point
 (sgm/modules/attention.py:457-460).  CUDA (= HIP) dispatch key only: a CPU tensor fails in the dispatcher.  The framework's own
