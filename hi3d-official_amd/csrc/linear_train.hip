@@ -7,6 +7,11 @@
 // contraction).  Here all three products read the tensors as a training step holds them: an operand is either contiguous along the
 // contraction (KC: x and w forward, dz for dx) or across it (KS: w for dx, both for dw), and a KS tile reaches the matrix instruction
 // through gfx950's transposing LDS read, so nothing is transposed in memory.
+//
+// Bound by the matrix instructions where the sizes allow: the K loop of the 256 x 320 tile runs at 1450 TFLOP/s with all CUs at work (the library's
+// product of 8192^3: 1407), LDS reads at 77 % of their rate beside it.  Measured, bf16: 16384 x 1280 -> 5120 forward 178 us (1206 TFLOP/s), dx 153
+// (1405), dw 190 (1130, its contraction split in 3); 65536 x 2560 -> 640 182; 8192^3 801 / 807 / 809; 2048 x 1024 -> 1024 10.2 (421); 16 rows
+// 1280 -> 1280 5.4 us, a launch.  What keeps the first from more is a tile's start and end (about 12 us, four rounds), with GELU about 14 us more.
 #include "train_common.h"
 
 namespace {
@@ -371,7 +376,8 @@ __device__ __forceinline__ void mat_tile(const MatParams& p, int bid, char* smem
   constexpr unsigned NONE = 0x80000000u;
   const int fr = lane & 15, fg = lane >> 4;
   const int cols = p.N - n0;                        // of the tile that exist
-  const bool fits = p.N % 8 == 0 && (!p.e.res || (p.e.ldr % 8 == 0 && p.e.ldr <= MOST_PITCH && ((unsigned long)p.e.res & 15) == 0));      // 16-byte accesses do
+  const bool fits = p.N % 8 == 0 && (((unsigned long)p.e.y | (unsigned long)p.e.z) & 15) == 0 &&
+                    (!p.e.res || (p.e.ldr % 8 == 0 && p.e.ldr <= MOST_PITCH && ((unsigned long)p.e.res & 15) == 0));      // 16-byte accesses do
   const bool wide = p.part || p.e.res || !fits;     // fp32 through LDS
   const int wrow = wm * 16 + fr, wcol = wn * 16 * NT + fg * 4;
   f32x4 bias[NT];
@@ -506,7 +512,8 @@ __global__ __launch_bounds__(WM * WN * 64, MT == 2 ? 4 : 2) void mat_kernel(cons
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   mat_tile<T, AKS, BKS, WM, WN, MT, NT>(p, blockIdx.x, smem);
 }
-// dw and dx of a layer in one launch, where neither fills the chip by itself: the first `first` blocks are dw's (the longer ones)
+// dw and dx of a layer in one launch, where neither fills the chip by itself (3083 x 650 -> 1290: 65 us one after the other, 46 with this and the
+// prepared operands in one launch too): the first `first` blocks are dw's (the longer ones)
 template <typename T, int WM, int WN, int MT, int NT>
 __global__ __launch_bounds__(WM * WN * 64, MT == 2 ? 4 : 2) void both_gradients_kernel(const MatParams dw, const MatParams dx, int first) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];

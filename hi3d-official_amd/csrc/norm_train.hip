@@ -11,7 +11,11 @@
 // large against its spread keeps its digits), all in fp32.
 //
 // A row is held by LPR lanes of a wave (8 ... 64) as NV vectors of 16 bytes each, so that a wave carries 64 / LPR rows at a
-// time and a row sum is log2(LPR) steps for all of them at once; wider rows are held by the block (LPR = 256).
+// time and a row sum is log2(LPR) steps for all of them at once; wider rows are held by the block (LPR = 256 or 512).
+//
+// Measured, bf16 rows with fp32 weights: residual sum + norm of 262144 x 320 126 us (5.3 TB/s; a copy of 2 GiB reaches 4.9), norm of 65536 x 640
+// 27.6 us (6.1 TB/s: half of it stays in the last-level cache), gradients of 65536 x 640 with the residual stream's 72 us (4.7 TB/s, 4 us of it the
+// columns' sums), of 7013 x 1285 fp16 22 us (2.4 TB/s: too few rows to hide a row's latency).
 #include "train_common.h"
 
 namespace {
@@ -371,7 +375,7 @@ int bwd_blocks(long R, int C, int dtype) {
   return (int)blocks_for(R, lpr, BWD_BLOCKS, bwd_rows(lpr));
 }
 
-int bad_sizes(const char* what, long R, int C, int dtype, int wcode) {
+int bad_sizes(long R, int C, int dtype, int wcode) {
   if (!hi3d_known_dtype(dtype) || !hi3d_known_dtype(wcode)) HI3D_FAIL(HI3D_EINVAL, "layernorm training: unknown element type");
   if (R < 0 || C <= 0) HI3D_FAIL(HI3D_EINVAL, "layernorm training: negative row count or width < 1");
   if (C > HI3D_NORM_MAX_WIDTH) HI3D_FAIL(HI3D_ESHAPE, "layernorm training: width over 8192");
@@ -388,7 +392,7 @@ int hi3d_column_reduce(const float* part, void* o0, void* o1, int code0, int cod
 
 extern "C" int hi3d_layernorm_fwd(const void* x, const void* residual, const void* weight, const void* bias, void* y, void* z, float* mean,
                                   float* rstd, int64_t R, int32_t C, int64_t ldx, int64_t ldr, int32_t dtype, int32_t wdtype, float eps, void* stream) {
-  if (const int rc = bad_sizes("fwd", R, C, dtype, wdtype)) return rc;
+  if (const int rc = bad_sizes(R, C, dtype, wdtype)) return rc;
   if (!(eps >= 0.0f) || eps > 3.0e38f) HI3D_FAIL(HI3D_EINVAL, "layernorm_fwd: eps must be finite and not negative");
   if (R == 0) return 0;
   if (!x || !y || !mean || !rstd || (residual && !z)) HI3D_FAIL(HI3D_EINVAL, "layernorm_fwd: null pointer");
@@ -407,7 +411,7 @@ extern "C" int64_t hi3d_layernorm_bwd_workspace_floats(int64_t R, int32_t C, int
 extern "C" int hi3d_layernorm_bwd(const void* dy, const void* z, const void* dz, const void* weight, const float* mean, const float* rstd, void* dx,
                                   void* dweight, void* dbias, float* ws, int64_t R, int32_t C, int64_t lddy, int64_t ldz, int64_t lddz, int32_t dtype,
                                   int32_t wdtype, void* stream) {
-  if (const int rc = bad_sizes("bwd", R, C, dtype, wdtype)) return rc;
+  if (const int rc = bad_sizes(R, C, dtype, wdtype)) return rc;
   const hipStream_t st = (hipStream_t)stream;
   if (R == 0) return (dweight || dbias) ? hi3d_column_reduce(nullptr, dweight, dbias, wdtype, wdtype, 0, C, 2 * C, st) : 0;   // sums of nothing
   if (!dy || !z || !mean || !rstd || !dx) HI3D_FAIL(HI3D_EINVAL, "layernorm_bwd: null pointer");

@@ -11,17 +11,17 @@ struct bf16_t { unsigned short u; };
 
 template <typename T> struct Elem;
 template <> struct Elem<float> {
-  static constexpr int VEC = 4, CODE = HI3D_F32;
+  static constexpr int VEC = 4;
   static __device__ __forceinline__ float get(float v) { return v; }
   static __device__ __forceinline__ float put(float v) { return v; }
 };
 template <> struct Elem<half_t> {
-  static constexpr int VEC = 8, CODE = HI3D_F16;
+  static constexpr int VEC = 8;
   static __device__ __forceinline__ float get(half_t v) { return (float)v; }
   static __device__ __forceinline__ half_t put(float v) { return (half_t)v; }      // round to nearest even, overflow to infinity
 };
 template <> struct Elem<bf16_t> {
-  static constexpr int VEC = 8, CODE = HI3D_BF16;
+  static constexpr int VEC = 8;
   static __device__ __forceinline__ float get(bf16_t v) { return bf16_to_f32(v.u); }
   static __device__ __forceinline__ bf16_t put(float v) { return bf16_t{f32_to_bf16(v)}; }
 };
@@ -115,12 +115,7 @@ __device__ __forceinline__ void load_vec_as(const void* p, int code, int e, int 
   else { Pack<half_t, N> k; fetch((const half_t*)p + e, n, e, k); unpack(k, f); }
 }
 
-// one element of a tensor whose type is known at run time only (weights, biases: read or written once per block)
-__device__ __forceinline__ float load_as(const void* p, int code, long i) {
-  if (code == HI3D_F32) return ((const float*)p)[i];
-  if (code == HI3D_BF16) return bf16_to_f32(((const unsigned short*)p)[i]);
-  return (float)((const half_t*)p)[i];
-}
+// one element of a tensor whose type is known at run time only (gradients of weights: written once)
 __device__ __forceinline__ void store_as(void* p, int code, long i, float v) {
   if (code == HI3D_F32) ((float*)p)[i] = v;
   else if (code == HI3D_BF16) ((unsigned short*)p)[i] = f32_to_bf16(v);
@@ -161,6 +156,5 @@ int hi3d_column_reduce(const float* part, void* o0, void* o1, int code0, int cod
 namespace {
 
 inline bool hi3d_known_dtype(int c) { return c == HI3D_F32 || c == HI3D_BF16 || c == HI3D_F16; }
-inline int hi3d_dtype_size(int c) { return c == HI3D_F32 ? 4 : 2; }
 
 }  // namespace

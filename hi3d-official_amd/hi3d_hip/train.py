@@ -187,18 +187,26 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As torch's, but the moments and copies keep their own types (torch casts a state to its parameter's type), and working
-        copies that have been handed out take the loaded values."""
+        copies that have been handed out take the loaded values.  A state of torch.optim.AdamW loads too."""
+        def keep(p, name, v):
+            with torch.no_grad():
+                to = copies[p] if name == "copy" and p in copies and copies[p].dtype == v.dtype else torch.empty_like(p, dtype=v.dtype, requires_grad=False)
+                to.copy_(v)
+            return to.requires_grad_(p.requires_grad) if name == "copy" else to
+
         copies = {p: s["copy"] for p, s in self.state.items() if "copy" in s}
         super().load_state_dict(state_dict)
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
-            for k, v in state_dict["state"].get(i, {}).items():
-                if torch.is_tensor(v):
-                    with torch.no_grad():
-                        to = copies[p] if k == "copy" and p in copies and copies[p].dtype == v.dtype else torch.empty_like(p, dtype=v.dtype, requires_grad=False)
-                        to.copy_(v)
-                    self.state[p][k] = to.requires_grad_(p.requires_grad) if k == "copy" else to
+            saved = state_dict["state"].get(i, {})
+            for k in ("exp_avg", "exp_avg_sq", "copy"):
+                if k in saved:
+                    self.state[p][k] = keep(p, k, saved[k].float() if k != "copy" else saved[k])
+            if "step" in saved:
+                self.state[p]["step"] = int(saved["step"])
         for g in self.param_groups:
+            for k, v in self.defaults.items():               # (a group saved by torch.optim.AdamW has no working_dtype)
+                g.setdefault(k, v)
             if g["step_t"] is not None and g["params"]:
                 g["step_t"] = g["step_t"].detach().clone().to(g["params"][0].device)
         self._step_supports_amp_scaling = all(g["capturable"] for g in self.param_groups)

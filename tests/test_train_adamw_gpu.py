@@ -215,6 +215,17 @@ def test_optimiser_is_torchs(dev):
     o.step()
     o2 = train.AdamW([b])
     o2.load_state_dict(o.state_dict())
+    t = torch.nn.Parameter(b.detach().float())                    # a state that torch's optimiser saved
+    ot = torch.optim.AdamW([t], lr=0.5, weight_decay=0.0)
+    t.grad = torch.ones_like(t)
+    ot.step()
+    u = torch.nn.Parameter(t.detach().clone())
+    o5 = train.AdamW([u])
+    o5.load_state_dict(ot.state_dict())
+    t.grad = u.grad = torch.full_like(t, 0.5)
+    ot.step(); o5.step()
+    assert o5.state[u]["step"] == 2 and o5.param_groups[0]["lr"] == 0.5
+    assert ((t - u).abs() <= 64 * U32 * (t.detach().abs() + 1)).all()          # (both in fp32: a step's roundings, above, on each side)
     w = torch.nn.Parameter(torch.randn(10, device=dev))
     o3, o4 = train.AdamW([w], working_dtype=torch.bfloat16), train.AdamW([w], working_dtype=torch.bfloat16)
     held = o4.working_copy(w)

@@ -180,6 +180,37 @@ def test_what_lies_around_the_operands_is_not_read_into_results(dev, ns):
         assert all(torch.equal(p, q) for p, q in zip(e, f))
 
 
+def test_results_at_any_alignment(dev, ns):
+    """The C entries' outputs (torch allocates aligned ones): one element off, and nothing around them is written."""
+    import ctypes as C
+    from hi3d_hip import lib as l
+    lib = l.load()
+
+    class Desc(C.Structure):
+        _fields_ = [(n, C.c_void_p) for n in ("x", "w", "bias", "residual", "y", "z", "dy", "dx", "dw", "db")] + \
+                   [(n, C.c_int64) for n in ("M", "ldx", "ldw", "ldr", "lddy", "ldz")] + [(n, C.c_int32) for n in ("N", "K", "dtype", "bias_dtype", "act")] + \
+                   [("ws", C.c_void_p), ("ws_bytes", C.c_int64)]
+    M, N, K = 200, 136, 72
+    x, w, b, dy, z = rnd((M, K), 1, "bf16").to(dev), rnd((N, K), 2, "bf16").to(dev), rnd((N,), 3).to(dev), rnd((M, N), 4, "bf16").to(dev), rnd((M, N), 5, "bf16").to(dev)
+    y0, z0 = ns.linear_act(x, w, b, None, "gelu", True)
+    g0 = ns.linear_act_bwd(dy, x, w, z, b, "gelu", True, True)
+    ws = torch.empty(1 << 24, dtype=torch.uint8, device=dev)
+    off = [torch.full((n + 9,), 7.0, dtype=torch.bfloat16, device=dev) for n in (M * N, M * N, M * K, N * K)]
+    p = [t.data_ptr() + 2 for t in off]
+    db = torch.empty(N, device=dev)
+    d = Desc(x=x.data_ptr(), w=w.data_ptr(), bias=b.data_ptr(), y=p[0], z=p[1], M=M, ldx=K, ldw=K, N=N, K=K, dtype=1, bias_dtype=0, act=1, ws=ws.data_ptr(), ws_bytes=ws.numel())
+    st = torch.cuda.current_stream().cuda_stream
+    assert lib.hi3d_linear_fwd(C.addressof(d), st) == 0
+    e = Desc(x=x.data_ptr(), w=w.data_ptr(), dy=dy.data_ptr(), z=z.data_ptr(), dx=p[2], dw=p[3], db=db.data_ptr(), M=M, ldx=K, ldw=K, lddy=N, ldz=N, N=N, K=K, dtype=1, bias_dtype=0,
+             act=1, ws=ws.data_ptr(), ws_bytes=ws.numel())
+    assert lib.hi3d_linear_bwd(C.addressof(e), st) == 0
+    torch.cuda.synchronize()
+    for t, want in zip(off, (y0, z0, g0[0], g0[1])):
+        n = want.numel()
+        assert torch.equal(t[1:1 + n].reshape(want.shape), want) and t[0] == 7 and (t[1 + n:] == 7).all()
+    assert torch.equal(db, g0[2])
+
+
 def test_rows_far_apart(dev, ns):
     """Pitches that a tile's 32-bit offsets do not reach, for every operand."""
     M, N, K, ld = 65, 72, 96, 3_000_000
