@@ -619,24 +619,27 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, Epilogue e
 
 // What the products need first, in one launch:
 //   dz = dy act'(z), rounded to the operands' type for the matrix instruction (its sums stay fp32), in rows padded with zeros to a multiple of 8
-//   elements; and the column sums of the unrounded dz, one row of partial sums per block row (256 columns x 8 row lanes a block);
+//   elements; and the column sums of the unrounded dz, one row of partial sums per block row (256 columns x 8 row lanes a block; up to SLOPE_FEW rows
+//   64 columns x 32 row lanes, and the sums themselves: one launch less);
 //   up to two operands whose rows cannot be read in place, padded likewise.
 struct SlopeParams {
   const void* dy; const void* z; void* dz; float* part;
   long M, lddy, ldz;
-  int N, act, rows;                        // rows: of a block
+  void* db;                                // instead of partial sums, where one block has all rows
+  int N, act, rows, db_code;               // rows: of a block
 };
+constexpr int SLOPE_FEW = 128;
 struct PadParams { const void* in; void* out; long rows, ld; int cols, blocks; };
 
-template <typename T>
-__device__ __forceinline__ void slope(const SlopeParams& p, int bx, int by) {
-  __shared__ float lds[8][256];
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, c = bx * 256 + tx * 8, n = p.N - c;
+template <typename T, int TX>
+__device__ __forceinline__ void slope(const SlopeParams& p, int bx, int by, float* lds) {
+  constexpr int COLS = TX * 8, TY = 256 / TX;
+  const int tx = threadIdx.x % TX, ty = threadIdx.x / TX, c = bx * COLS + tx * 8, n = p.N - c;
   const long r0 = (long)by * p.rows, r1 = min(p.M, r0 + p.rows);
   const long ldo = (p.N + 7) / 8 * 8;
   float s[8] = {};
   if (n > 0)
-    for (long r = r0 + ty; r < r1; r += 8) {
+    for (long r = r0 + ty; r < r1; r += TY) {
       Pack<T, 8> ky, kz;
       float v[8], z[8];
       fetch((const T*)p.dy + r * p.lddy + c, n, c, ky);
@@ -654,23 +657,24 @@ __device__ __forceinline__ void slope(const SlopeParams& p, int bx, int by) {
       for (int j = 0; j < 8; ++j) s[j] += v[j];
       if (p.dz) store_some((T*)p.dz + r * ldo + c, 8, v);
     }
-  if (!p.part) return;
+  if (!p.part && !p.db) return;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) lds[ty][tx * 8 + j] = s[j];
+  for (int j = 0; j < 8; ++j) lds[ty * COLS + tx * 8 + j] = s[j];
   __syncthreads();
-  const int col = bx * 256 + threadIdx.x;
-  if (col < p.N) {
+  const int col = bx * COLS + threadIdx.x;
+  if (threadIdx.x < COLS && col < p.N) {
     float t = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) t += lds[k][threadIdx.x];
-    p.part[(long)by * p.N + col] = t;
+    for (int k = 0; k < TY; ++k) t += lds[k * COLS + threadIdx.x];
+    if (p.db) store_as(p.db, p.db_code, col, t);
+    else p.part[(long)by * p.N + col] = t;
   }
 }
 template <typename T>
 __device__ __forceinline__ void pad_rows(const PadParams& p, int block) {
   const int cpr = (p.cols + 7) / 8;
   for (long c = (long)block * 256 + threadIdx.x; c < p.rows * cpr; c += (long)p.blocks * 256) {
-    const long r = c / cpr;
+    const long r = (c >> 32) ? c / cpr : (long)((unsigned)c / (unsigned)cpr);
     const int e = (int)(c - r * cpr) * 8;
     Pack<T, 8> k;
     fetch((const T*)p.in + r * p.ld + e, p.cols - e, e, k);
@@ -679,8 +683,12 @@ __device__ __forceinline__ void pad_rows(const PadParams& p, int block) {
 }
 template <typename T>
 __global__ __launch_bounds__(256) void prepare_kernel(const SlopeParams s, int across, int slope_blocks, const PadParams a, const PadParams b) {
+  __shared__ float lds[2048];
   const int bid = blockIdx.x;
-  if (bid < slope_blocks) slope<T>(s, bid % across, bid / across);
+  if (bid < slope_blocks) {
+    if (s.M <= SLOPE_FEW) slope<T, 8>(s, bid, 0, lds);
+    else slope<T, 32>(s, bid % across, bid / across, lds);
+  }
   else if (bid < slope_blocks + a.blocks) pad_rows<T>(a, bid - slope_blocks);
   else pad_rows<T>(b, bid - slope_blocks - a.blocks);
 }
@@ -796,13 +804,13 @@ Operand place(const void* p, long rows, int cols, long ld, char** ws, PadParams*
   if (in_place(p, ld, cols)) return {p, ld};
   char* const to = *ws;
   *ws += padded_bytes(rows, cols);
-  const long blocks = (rows * ((cols + 7L) / 8) + 1023) / 1024;
-  *job = {p, to, rows, ld, cols, (int)(blocks < 4096 ? blocks : 4096)};
+  const long blocks = (rows * ((cols + 7L) / 8) + 255) / 256;             // (a chunk a thread while that fills the chip: each is a trip to memory)
+  *job = {p, to, rows, ld, cols, (int)(blocks < 8192 ? blocks : 8192)};
   return {to, (cols + 7L) / 8 * 8};
 }
 template <typename T>
 int prepare(const SlopeParams& s, int slices, const PadParams& a, const PadParams& b, hipStream_t st) {
-  const int across = (s.N + 255) / 256, n = across * slices;
+  const int cols = s.M <= SLOPE_FEW ? 64 : 256, across = (s.N + cols - 1) / cols, n = across * slices;
   if (n + a.blocks + b.blocks == 0) return 0;
   hipLaunchKernelGGL((prepare_kernel<T>), dim3((unsigned)(n + a.blocks + b.blocks)), dim3(256), 0, st, s, across > 0 ? across : 1, n, a, b);
   HI3D_LAUNCH_CHECK();
@@ -811,6 +819,7 @@ int prepare(const SlopeParams& s, int slices, const PadParams& a, const PadParam
 
 constexpr int SLOPE_BLOCKS = 2048;
 int slope_rows(long M, int N) {
+  if (M <= SLOPE_FEW) return SLOPE_FEW;
   const long cols = (N + 255) / 256, want = SLOPE_BLOCKS / cols > 0 ? SLOPE_BLOCKS / cols : 1;
   long rows = (M + want - 1) / want;
   rows = rows < 32 ? 32 : (rows + 7) / 8 * 8;
@@ -880,7 +889,7 @@ BwdNeeds bwd_needs(const hi3d_linear_desc* d) {
   }
   const long a = d->dx ? part_bytes(n.dx, d->M, d->K) : 0, b = d->dw ? part_bytes(n.dw, d->N, d->K) : 0;
   n.part = a > b ? a : b;
-  if (d->db) n.cols = round256((long)slope_slices(d->M, d->N) * d->N * 4);
+  if (d->db && d->M > SLOPE_FEW) n.cols = round256((long)slope_slices(d->M, d->N) * d->N * 4);
   return n;
 }
 
@@ -912,16 +921,17 @@ int bwd(const hi3d_linear_desc* d, hipStream_t st) {
   const BwdNeeds n = bwd_needs(d);
   char* ws = (char*)d->ws;
   Operand dz = {d->dy, (long)d->lddy};
-  SlopeParams sp = {d->dy, d->z, nullptr, nullptr, (long)d->M, (long)d->lddy, (long)d->ldz, d->N, d->act, slope_rows(d->M, d->N)};
+  SlopeParams sp = {d->dy, d->z, nullptr, nullptr, (long)d->M, (long)d->lddy, (long)d->ldz, nullptr, d->N, d->act, slope_rows(d->M, d->N), d->bias_dtype};
   if (n.dz) { sp.dz = ws; dz = {ws, (d->N + 7L) / 8 * 8}; ws += n.dz; }
-  if (d->db) { sp.part = (float*)ws; ws += n.cols; }
+  if (n.cols) { sp.part = (float*)ws; ws += n.cols; }
+  else sp.db = d->db;
   const int slices = (n.dz || d->db) ? slope_slices(d->M, d->N) : 0;
   PadParams jw = {}, jx = {};
   Operand w = {}, x = {};
   if (d->dx) w = place(d->w, d->N, d->K, d->ldw, &ws, &jw);
   if (d->dw) x = place(d->x, d->M, d->K, d->ldx, &ws, &jx);
   if (const int rc = prepare<T>(sp, slices, jw, jx, st)) return rc;
-  if (d->db)
+  if (sp.part)
     if (const int rc = hi3d_column_reduce(sp.part, d->db, nullptr, d->bias_dtype, 0, slices, d->N, d->N, st)) return rc;
   float* const part = (float*)ws;                   // (dx's and dw's in turn: they follow each other on the stream, and in one launch only dw is split)
   MatParams px = {}, pw = {};

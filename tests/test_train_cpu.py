@@ -76,8 +76,8 @@ def test_linear_refuses(lib, k):
     assert lib.hi3d_linear_fwd(C.addressof(d), 0) < 0 and lib.hi3d_last_error()
 
 
-@pytest.mark.parametrize("k", [dict(dy=0), dict(x=0), dict(w=0), dict(act=1), dict(act=1, z=P, ldz=63), dict(lddy=63), dict(ldx=63), dict(ldw=63), dict(db=P, ws=0), dict(M=1 << 31),
-                               dict(act=1, z=P, ws_bytes=64 * 64 * 2)])
+@pytest.mark.parametrize("k", [dict(dy=0), dict(x=0), dict(w=0), dict(act=1), dict(act=1, z=P, ldz=63), dict(lddy=63), dict(ldx=63), dict(ldw=63), dict(M=129, db=P, ws=0), dict(M=1 << 31),
+                               dict(act=1, z=P, ws_bytes=64 * 64 * 2 - 1)])
 def test_linear_bwd_refuses(lib, k):
     d = linear(**k)
     assert lib.hi3d_linear_bwd(C.addressof(d), 0) < 0 and lib.hi3d_last_error()

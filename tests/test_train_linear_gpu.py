@@ -84,7 +84,7 @@ def check_bwd(ns, dy, x, w, z, b, act):
             db = got[2]
 
 
-SIZES = [(1, 1, 1), (1, 8, 8), (2, 3, 5), (7, 64, 64), (16, 1280, 320), (33, 40, 72), (64, 64, 129), (100, 130, 70), (129, 257, 65), (257, 321, 193), (300, 320, 640),
+SIZES = [(1, 1, 1), (1, 8, 8), (2, 3, 5), (7, 64, 64), (16, 1280, 320), (33, 40, 72), (64, 64, 129), (100, 130, 70), (128, 66, 24), (129, 257, 65), (257, 321, 193), (300, 320, 640),
          (513, 640, 136), (1, 1280, 5120), (4, 37, 4101), (7, 50, 2055), (8, 24, 4999), (17, 1290, 650), (32, 33, 1029)]
 
 
