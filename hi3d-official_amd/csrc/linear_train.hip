@@ -108,7 +108,7 @@ __device__ __forceinline__ void finish(const Epilogue& e, long m, int c, int n, 
 // that is a multiple of 8 elements, 16-byte aligned; a row of KC holds zeros from K up to the next multiple of 8.
 struct MatParams {
   const char* A; const char* B;
-  float* part;            // split contraction: partial sums [split][M][N]; NULL: the epilogue below
+  float* part;            // split contraction: partial sums [split][M][N rounded up to 8]; NULL: the epilogue below
   Epilogue e;
   long lda, ldb;
   int M, N, K, nbm, nbn, splits, per;      // per: K steps of a split
@@ -375,7 +375,7 @@ __device__ __forceinline__ void mat_tile(const MatParams& p, int bid, char* smem
   static_assert(2 * (FSLAB + HSLAB) <= 2 * STAGE, "two buffers of both kinds fit the tiles' LDS");
   constexpr unsigned NONE = 0x80000000u;
   const int fr = lane & 15, fg = lane >> 4;
-  const int cols = p.N - n0;                        // of the tile that exist
+  const int width = p.part ? (p.N + 7) & ~7 : p.N, cols = width - n0;           // columns of the tile that exist (partial sums: in whole chunks)
   const bool fits = p.N % 8 == 0 && (((unsigned long)p.e.y | (unsigned long)p.e.z) & 15) == 0 &&
                     (!p.e.res || (p.e.ldr % 8 == 0 && p.e.ldr <= MOST_PITCH && ((unsigned long)p.e.res & 15) == 0));      // 16-byte accesses do
   const bool wide = p.part || p.e.res || !fits;     // fp32 through LDS
@@ -384,7 +384,7 @@ __device__ __forceinline__ void mat_tile(const MatParams& p, int bid, char* smem
 #pragma unroll
   for (int j = 0; j < NT; ++j) bias[j] = *(const f32x4*)(smem + 2 * STAGE + (wcol + j * 16) * 4);
   const int esz = p.part ? 4 : 2;
-  const long ldo = p.part ? p.N : p.e.ldo;
+  const long ldo = p.part ? width : p.e.ldo;
   unsigned off[CH], roff[CH];                       // of the thread's chunks of 8 columns: bytes in the output and the residual, the LDS places
   int hat[CH], fat[CH];
 #pragma unroll
@@ -445,8 +445,8 @@ __device__ __forceinline__ void mat_tile(const MatParams& p, int bid, char* smem
       }
       meet();
       if constexpr (ACT < 0) {
-        if (p.part && p.N % 8 == 0) {
-          const __amdgpu_buffer_rsrc_t to = window(p.part + (long)ks * p.M * p.N, ldo, 4, i);
+        if (p.part) {
+          const __amdgpu_buffer_rsrc_t to = window(p.part + (long)ks * p.M * width, ldo, 4, i);
 #pragma unroll
           for (int t = 0; t < CH; ++t) {
             __builtin_amdgcn_raw_buffer_store_b128(*(const u32x4*)(fslab + fat[t]), to, off[t], 0, 0);
@@ -460,8 +460,7 @@ __device__ __forceinline__ void mat_tile(const MatParams& p, int bid, char* smem
             if (m >= p.M || q * 8 >= cols) continue;
             const f32x4 lo = *(const f32x4*)(fslab + r * FROW + q * 16), hi = *(const f32x4*)(fslab + r * FROW + q * 16 + CPR * 16);
             float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-            if (p.part) store_some(p.part + ((long)ks * p.M + m) * p.N + n, p.N - n, v);
-            else finish<T>(p.e, m, n, p.N - n, v);
+            finish<T>(p.e, m, n, p.N - n, v);
           }
         }
       } else {
@@ -598,22 +597,37 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void few_rows_kernel(const FewParam
 #endif
 }
 
-// the partial sums of a split contraction, in the order of the splits, and the epilogue
-template <typename T>
+// The partial sums of a split contraction and the epilogue.  G threads take every G-th split of a chunk of 8 columns each, and their sums are added in
+// their order: many splits of a small output would otherwise be as many trips to memory, one after the other (31 splits of 3 x 480: 6.5 us).
+template <typename T, int G>
 __global__ __launch_bounds__(256) void join_kernel(const float* part, Epilogue e, long M, int N, int splits) {
-  const int cpr = (N + 7) / 8;
-  for (long c = (long)blockIdx.x * 256 + threadIdx.x; c < M * cpr; c += (long)gridDim.x * 256) {
-    const long m = c / cpr;
+  constexpr int CHUNKS = 256 / G;
+  __shared__ float sums[G > 1 ? G : 1][G > 1 ? CHUNKS : 1][9];
+  const int cpr = (N + 7) / 8, g = threadIdx.x / CHUNKS, t = threadIdx.x % CHUNKS;
+  for (long c0 = (long)blockIdx.x * CHUNKS; c0 < M * cpr; c0 += (long)gridDim.x * CHUNKS) {
+    const long c = c0 + t, m = c / cpr;
     const int n = (int)(c - m * cpr) * 8;
     float v[8] = {};
+    if (m < M) {
 #pragma unroll 4
-    for (int s = 0; s < splits; ++s) {
-      Pack<float, 8> k;
-      fetch(part + (s * M + m) * N + n, N - n, n, k);
+      for (int s = g; s < splits; s += G) {
+        const Pack<float, 8> k = *(const Pack<float, 8>*)(part + (s * M + m) * (cpr * 8L) + n);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += __uint_as_float(k.w[j]);
+        for (int j = 0; j < 8; ++j) v[j] += __uint_as_float(k.w[j]);
+      }
     }
-    finish<T>(e, m, n, N - n, v);
+    if constexpr (G > 1) {
+      __syncthreads();                              // (the last chunk's sums have been read)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sums[g][t][j] = v[j];
+      __syncthreads();
+      if (g) continue;
+#pragma unroll
+      for (int k = 1; k < G; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += sums[k][t][j];
+    }
+    if (m < M) finish<T>(e, m, n, N - n, v);
   }
 }
 
@@ -747,7 +761,7 @@ BothPlan both_plan_of(long M, long N, long K, const Plan& dx, const Plan& dw) {
 }
 
 long round256(long b) { return (b + 255) & ~255L; }
-long part_bytes(const Plan& p, long M, long N) { return p.splits > 1 ? round256(p.splits * M * N * 4) : 0; }
+long part_bytes(const Plan& p, long M, long N) { return p.splits > 1 ? round256(p.splits * M * ((N + 7) / 8 * 8) * 4) : 0; }
 
 template <typename T, bool AKS, bool BKS, int WM, int WN, int MT, int NT>
 int launch_cfg(const MatParams& p, hipStream_t st) {
@@ -769,7 +783,9 @@ void set_plan(MatParams* p, const Plan& plan, float* part) {
 template <typename T>
 int join(const MatParams& p, hipStream_t st) {
   if (p.splits == 1) return 0;
-  hipLaunchKernelGGL((join_kernel<T>), dim3(grid_of((long)p.M * ((p.N + 7) / 8))), dim3(256), 0, st, (const float*)p.part, p.e, (long)p.M, p.N, p.splits);
+  const long chunks = (long)p.M * ((p.N + 7) / 8);
+  if (p.splits >= 8) hipLaunchKernelGGL((join_kernel<T, 8>), dim3(grid_of(chunks * 8)), dim3(256), 0, st, (const float*)p.part, p.e, (long)p.M, p.N, p.splits);
+  else hipLaunchKernelGGL((join_kernel<T, 1>), dim3(grid_of(chunks)), dim3(256), 0, st, (const float*)p.part, p.e, (long)p.M, p.N, p.splits);
   HI3D_LAUNCH_CHECK();
   return 0;
 }
@@ -987,8 +1003,8 @@ extern "C" int hi3d_linear_bwd(const hi3d_linear_desc* d, void* stream) {
     if (d->dw) {
       const Epilogue e = {nullptr, nullptr, d->dw, nullptr, 0, (long)d->K, HI3D_F32, HI3D_ACT_NONE};
       const dim3 grid(grid_of((long)d->N * ((d->K + 7) / 8)));
-      if (d->dtype == HI3D_BF16) hipLaunchKernelGGL((join_kernel<bf16_t>), grid, dim3(256), 0, st, nullptr, e, (long)d->N, d->K, 0);
-      else hipLaunchKernelGGL((join_kernel<half_t>), grid, dim3(256), 0, st, nullptr, e, (long)d->N, d->K, 0);
+      if (d->dtype == HI3D_BF16) hipLaunchKernelGGL((join_kernel<bf16_t, 1>), grid, dim3(256), 0, st, nullptr, e, (long)d->N, d->K, 0);
+      else hipLaunchKernelGGL((join_kernel<half_t, 1>), grid, dim3(256), 0, st, nullptr, e, (long)d->N, d->K, 0);
       HI3D_LAUNCH_CHECK();
     }
     return 0;
