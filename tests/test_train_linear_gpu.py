@@ -136,6 +136,14 @@ def test_activation_tails(dev, ns):
         near(y, ACTS[act](v.double()), 1e-5 * ACTS[act](v.double()).abs(), act)
         db = ns.linear_act_bwd(torch.ones_like(v).to(dev), v.to(dev), eye.to(dev), v.to(dev), None, act, True, False)[0].cpu()
         near(db, slope64(v.double(), act), 2e-5 * torch.ones(64, 64, dtype=torch.float64), act + "'")
+    odd = torch.tensor([[float("inf"), float("nan"), 0.5, -3.0, 0.0, 0.0, 0.0, 0.0]]).half()
+    for act in ("gelu", "quick_gelu", "silu", "relu"):                # one such value makes its whole row's sums of it: row by row, through a column of ones
+        for v0 in (odd[0, 0], odd[0, 1], -odd[0, 0]):
+            x1 = torch.zeros(1, 8, dtype=torch.float16)
+            x1[0, 0] = v0
+            y, z = (t.cpu() for t in ns.linear_act(x1.to(dev), torch.ones(8, 8, dtype=torch.float16, device=dev), None, None, act, True))
+            assert torch.equal(torch.isnan(z), torch.isnan(v0).expand(1, 8)) and (torch.isnan(v0) or (z == v0).all())
+            assert (torch.isnan(y) if torch.isnan(v0) else (y == v0) if v0 > 0 else (torch.isnan(y) | (y == 0))).all()
     big = torch.tensor([[1000.0, -1000.0, 60000.0, -60000.0, 0.0, -0.0, 1e-7, -1e-7]]).half()
     for act in ("gelu", "quick_gelu", "silu", "relu"):
         y, _ = ns.linear_act(big.to(dev), torch.eye(8, dtype=torch.float16, device=dev), None, None, act, False)
