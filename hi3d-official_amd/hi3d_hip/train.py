@@ -90,7 +90,7 @@ class AdamW(torch.optim.Optimizer):
     weights that the forward pass reads, `working_copy(p)`, a leaf with a gradient of its own: step() takes that one where p has none.
     capturable: step count on the device (per group: each of its parameters then needs a gradient at every step), so that step() can be
     captured into a HIP graph; `lr` may then be a one-element fp32 device tensor.  torch.amp.GradScaler's scale and
-    overflow flag are read on the device in this mode.
+    overflow flag are read on the device in this mode (it looks at the parameters' own gradients: not together with working copies').
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, working_dtype=None, capturable=False):
@@ -194,6 +194,9 @@ class AdamW(torch.optim.Optimizer):
                 to.copy_(v)
             return to.requires_grad_(p.requires_grad) if name == "copy" else to
 
+        for g in state_dict["param_groups"]:
+            if g.get("amsgrad") or g.get("maximize"):
+                raise _l.Hi3dError("a state with amsgrad or maximize cannot be continued here")
         copies = {p: s["copy"] for p, s in self.state.items() if "copy" in s}
         super().load_state_dict(state_dict)
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]

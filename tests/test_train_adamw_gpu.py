@@ -222,6 +222,8 @@ def test_optimiser_is_torchs(dev):
     u = torch.nn.Parameter(t.detach().clone())
     o5 = train.AdamW([u])
     o5.load_state_dict(ot.state_dict())
+    with pytest.raises(RuntimeError):
+        train.AdamW([u]).load_state_dict(torch.optim.AdamW([u], amsgrad=True).state_dict())
     t.grad = u.grad = torch.full_like(t, 0.5)
     ot.step(); o5.step()
     assert o5.state[u]["step"] == 2 and o5.param_groups[0]["lr"] == 0.5
