@@ -186,30 +186,44 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        """As torch's, but the moments and copies keep their own types (torch casts a state to its parameter's type), and working
-        copies that have been handed out take the loaded values.  A state of torch.optim.AdamW loads too."""
-        def keep(p, name, v):
-            with torch.no_grad():
-                to = copies[p] if name == "copy" and p in copies and copies[p].dtype == v.dtype else torch.empty_like(p, dtype=v.dtype, requires_grad=False)
-                to.copy_(v)
-            return to.requires_grad_(p.requires_grad) if name == "copy" else to
-
-        for g in state_dict["param_groups"]:
+        """As torch's, but the moments keep their type (torch casts a state to its parameter's), `working_dtype` and `capturable` stay as
+        this optimiser was made with them, and what it holds already -- moments, working copies, step counts and rates on the device -- is
+        filled in place: copies that were handed out and a step that was captured go on from the loaded values.  A state of
+        torch.optim.AdamW loads too; a copy that the state has not is its parameter, rounded (load the parameters first)."""
+        own = [(g["working_dtype"], g["capturable"], g["step_t"], g["lr"]) for g in self.param_groups]
+        held = {p: dict(s) for p, s in self.state.items()}
+        state, counts = state_dict["state"], []
+        for i, g in enumerate(state_dict["param_groups"]):
             if g.get("amsgrad") or g.get("maximize"):
                 raise _l.Hi3dError("a state with amsgrad or maximize cannot be continued here")
-        copies = {p: s["copy"] for p, s in self.state.items() if "copy" in s}
+            if g.get("step_t") is not None:
+                steps = [int(g["step_t"])] * len(g["params"])
+            else:
+                steps = [int(state.get(k, {}).get("step", 0)) for k in g["params"]]
+            if i < len(own) and own[i][1] and len(set(steps)) > 1:
+                raise _l.Hi3dError("capturable: every parameter of the group needs the same number of steps behind it")
+            counts.append(steps)
         super().load_state_dict(state_dict)
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
-            saved = state_dict["state"].get(i, {})
-            for k in ("exp_avg", "exp_avg_sq", "copy"):
-                if k in saved:
-                    self.state[p][k] = keep(p, k, saved[k].float() if k != "copy" else saved[k])
-            if "step" in saved:
-                self.state[p]["step"] = int(saved["step"])
-        for g in self.param_groups:
+        for g, saved_group, steps, (working_dtype, capturable, step_t, lr) in zip(self.param_groups, state_dict["param_groups"], counts, own):
             for k, v in self.defaults.items():               # (a group saved by torch.optim.AdamW has no working_dtype)
                 g.setdefault(k, v)
-            if g["step_t"] is not None and g["params"]:
-                g["step_t"] = g["step_t"].detach().clone().to(g["params"][0].device)
+            g["working_dtype"], g["capturable"], g["step_t"] = working_dtype, capturable, None
+            g["lr"] = lr.fill_(float(g["lr"])) if torch.is_tensor(lr) else float(g["lr"])
+            if capturable and steps and (step_t is not None or steps[0]):
+                g["step_t"] = torch.zeros(1, device=g["params"][0].device) if step_t is None else step_t
+                g["step_t"].fill_(float(steps[0]))
+            for p, k, step in zip(g["params"], saved_group["params"], steps):
+                saved, before = state.get(k, {}), held.get(p, {})
+                if not saved and not before:
+                    continue
+                s = self.state[p]
+                s["step"] = 0 if capturable else step
+                for name in ("exp_avg", "exp_avg_sq"):
+                    s[name] = before[name] if name in before else torch.zeros_like(p, dtype=torch.float32)
+                    s[name].copy_(saved[name]) if name in saved else s[name].zero_()
+                s.pop("copy", None)
+                if working_dtype is not None:
+                    s["copy"] = before["copy"] if "copy" in before else p.detach().to(working_dtype).requires_grad_(p.requires_grad)
+                    with torch.no_grad():
+                        s["copy"].copy_(saved["copy"] if "copy" in saved and saved["copy"].dtype == working_dtype else p)
         self._step_supports_amp_scaling = all(g["capturable"] for g in self.param_groups)

@@ -238,6 +238,60 @@ def test_optimiser_is_torchs(dev):
     assert o2.state[b]["exp_avg"].dtype == torch.float32 and torch.equal(o2.state[b]["exp_avg"], o.state[b]["exp_avg"]) and o2.state[b]["step"] == 1
 
 
+def test_optimiser_state_between_its_modes(dev):
+    """A state goes from host to device counts and back with its step count, and what the optimiser has handed out stays in use."""
+    from hi3d_hip import train
+    gen = torch.Generator().manual_seed(29)
+    start = torch.randn(300, generator=gen).to(dev)
+    grads = [torch.randn(300, generator=gen).to(dev) for _ in range(6)]
+
+    def take(opt, p, i):
+        p.grad = grads[i].clone()
+        opt.step()
+
+    a = torch.nn.Parameter(start.clone())                  # six steps without a break
+    whole = train.AdamW([a], lr=1e-2)
+    for i in range(6):
+        take(whole, a, i)
+
+    b = torch.nn.Parameter(start.clone())                  # host counts, device counts, host counts: two steps each
+    first = train.AdamW([b], lr=1e-2)
+    take(first, b, 0); take(first, b, 1)
+    second = train.AdamW([b], lr=torch.full((1,), 0.5, device=dev), capturable=True)
+    lr = second.param_groups[0]["lr"]
+    second.load_state_dict(first.state_dict())
+    group = second.param_groups[0]
+    assert group["capturable"] and group["lr"] is lr and abs(float(lr) - 1e-2) < 1e-8 and int(group["step_t"]) == 2
+    take(second, b, 2); take(second, b, 3)
+    third = train.AdamW([b], lr=0.5)
+    third.load_state_dict(second.state_dict())
+    assert not third.param_groups[0]["capturable"] and third.state[b]["step"] == 4
+    take(third, b, 4); take(third, b, 5)
+    # lr from fp32 device memory is off by half a step, relative: the rest is a step's roundings, 40 U of its change and 4 U of p
+    assert ((a - b).detach().abs() <= 6 * 128 * U32 * (a.detach().abs() + 6e-2 * 3)).all()
+
+    # buffers that are held are filled, not replaced; a state without copies gives the parameter, rounded
+    c = torch.nn.Parameter(start.clone())
+    opt = train.AdamW([c], working_dtype=torch.bfloat16, capturable=True)
+    copy = opt.working_copy(c)
+    copy.grad = grads[0].bfloat16()
+    opt.step()
+    state, count = dict(opt.state[c]), opt.param_groups[0]["step_t"]
+    with torch.no_grad():
+        c.copy_(b)
+    opt.load_state_dict(third.state_dict())
+    assert opt.working_copy(c) is copy and torch.equal(copy, b.bfloat16()) and opt.param_groups[0]["step_t"] is count and int(count) == 6
+    for k in ("exp_avg", "exp_avg_sq"):
+        assert opt.state[c][k] is state[k] and torch.equal(state[k], third.state[b][k])
+
+    # different counts cannot be kept as one on the device
+    p = [torch.nn.Parameter(start.clone()) for _ in range(2)]
+    uneven = train.AdamW(p)
+    take(uneven, p[0], 0)
+    with pytest.raises(RuntimeError):
+        train.AdamW(p, capturable=True).load_state_dict(uneven.state_dict())
+
+
 def test_optimiser_with_working_copies_captured(dev):
     from hi3d_hip import train
     p = [torch.nn.Parameter(torch.randn(n, device=dev)) for n in (10, 4100)]
