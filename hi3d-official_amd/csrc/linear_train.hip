@@ -865,6 +865,13 @@ const char* bad_desc(const hi3d_linear_desc* d) {
   if (d->act < HI3D_ACT_NONE || d->act > HI3D_ACT_RELU) return "linear training: unknown activation";
   return nullptr;
 }
+// An operand of one row has no pitch: whatever the caller gave, its width stands in for it.  What lies behind the last row of a contraction is kept out by
+// its distance from the descriptor's range, so that a pitch under the width would have read the one row again for every row behind it.
+hi3d_linear_desc one_row_pitches(hi3d_linear_desc d) {
+  if (d.M == 1) { d.ldx = d.K; d.ldr = d.lddy = d.ldz = d.N; }
+  if (d.N == 1) d.ldw = d.K;
+  return d;
+}
 bool too_big(const hi3d_linear_desc* d) { return d->M > 0x7fff0000L || d->N > MOST_WIDTH || d->K > MOST_WIDTH; }
 
 // Up to 32 rows the weights are streamed by few_rows_kernel, above that the tiles are faster (N = K = 4096, 32 / 48 / 65 rows: streamed 14 /
@@ -984,31 +991,35 @@ int bwd(const hi3d_linear_desc* d, hipStream_t st) {
 
 }  // namespace
 
-extern "C" int64_t hi3d_linear_fwd_workspace_bytes(const hi3d_linear_desc* d) {
-  if (bad_desc(d) || too_big(d) || d->M == 0) return 0;
-  const FwdNeeds n = fwd_needs(d);
+extern "C" int64_t hi3d_linear_fwd_workspace_bytes(const hi3d_linear_desc* desc) {
+  if (bad_desc(desc) || too_big(desc) || desc->M == 0) return 0;
+  const hi3d_linear_desc d = one_row_pitches(*desc);
+  const FwdNeeds n = fwd_needs(&d);
   return n.x + n.w + n.part;
 }
 
-extern "C" int hi3d_linear_fwd(const hi3d_linear_desc* d, void* stream) {
-  if (const char* why = bad_desc(d)) HI3D_FAIL(HI3D_EINVAL, why);
+extern "C" int hi3d_linear_fwd(const hi3d_linear_desc* desc, void* stream) {
+  if (const char* why = bad_desc(desc)) HI3D_FAIL(HI3D_EINVAL, why);
+  const hi3d_linear_desc local = one_row_pitches(*desc), *const d = &local;
   if (too_big(d)) HI3D_FAIL(HI3D_ESHAPE, "linear_fwd: a width is over 1048576, or too many rows");
   if (d->M == 0) return 0;
   if (!d->x || !d->w || !d->y) HI3D_FAIL(HI3D_EINVAL, "linear_fwd: null pointer");
-  if ((d->M > 1 && (d->ldx < d->K || (d->residual && d->ldr < d->N))) || (d->N > 1 && d->ldw < d->K)) HI3D_FAIL(HI3D_EINVAL, "linear_fwd: row pitch below the width");
+  if (d->ldx < d->K || (d->residual && d->ldr < d->N) || d->ldw < d->K) HI3D_FAIL(HI3D_EINVAL, "linear_fwd: row pitch below the width");
   const int64_t need = hi3d_linear_fwd_workspace_bytes(d);
   if (need && (!d->ws || d->ws_bytes < need || ((uintptr_t)d->ws & 255))) HI3D_FAIL(HI3D_EINVAL, "linear_fwd: workspace missing, too small or not 256-byte aligned");
   return d->dtype == HI3D_BF16 ? fwd<bf16_t>(d, (hipStream_t)stream) : fwd<half_t>(d, (hipStream_t)stream);
 }
 
-extern "C" int64_t hi3d_linear_bwd_workspace_bytes(const hi3d_linear_desc* d) {
-  if (bad_desc(d) || too_big(d) || d->M == 0) return 0;
-  const BwdNeeds n = bwd_needs(d);
+extern "C" int64_t hi3d_linear_bwd_workspace_bytes(const hi3d_linear_desc* desc) {
+  if (bad_desc(desc) || too_big(desc) || desc->M == 0) return 0;
+  const hi3d_linear_desc d = one_row_pitches(*desc);
+  const BwdNeeds n = bwd_needs(&d);
   return n.dz + n.x + n.w + n.cols + n.part;
 }
 
-extern "C" int hi3d_linear_bwd(const hi3d_linear_desc* d, void* stream) {
-  if (const char* why = bad_desc(d)) HI3D_FAIL(HI3D_EINVAL, why);
+extern "C" int hi3d_linear_bwd(const hi3d_linear_desc* desc, void* stream) {
+  if (const char* why = bad_desc(desc)) HI3D_FAIL(HI3D_EINVAL, why);
+  const hi3d_linear_desc local = one_row_pitches(*desc), *const d = &local;
   if (too_big(d)) HI3D_FAIL(HI3D_ESHAPE, "linear_bwd: a width is over 1048576, or too many rows");
   const hipStream_t st = (hipStream_t)stream;
   if (d->M == 0) {                       // sums over no rows
@@ -1024,7 +1035,7 @@ extern "C" int hi3d_linear_bwd(const hi3d_linear_desc* d, void* stream) {
     return 0;
   }
   if (!d->dy || (d->dx && !d->w) || (d->dw && !d->x) || (d->act != HI3D_ACT_NONE && !d->z)) HI3D_FAIL(HI3D_EINVAL, "linear_bwd: null pointer");
-  if ((d->M > 1 && (d->lddy < d->N || (d->act != HI3D_ACT_NONE && d->ldz < d->N) || (d->dw && d->ldx < d->K))) || (d->dx && d->N > 1 && d->ldw < d->K))
+  if (d->lddy < d->N || (d->act != HI3D_ACT_NONE && d->ldz < d->N) || (d->dw && d->ldx < d->K) || (d->dx && d->ldw < d->K))
     HI3D_FAIL(HI3D_EINVAL, "linear_bwd: row pitch below the width");
   const int64_t need = hi3d_linear_bwd_workspace_bytes(d);
   if (need && (!d->ws || d->ws_bytes < need || ((uintptr_t)d->ws & 255))) HI3D_FAIL(HI3D_EINVAL, "linear_bwd: workspace missing, too small or not 256-byte aligned");

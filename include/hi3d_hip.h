@@ -351,6 +351,7 @@ int hi3d_layernorm_bwd(const void* dy, const void* z, const void* dz, const void
  *        dz is rounded to `dtype` for the products (their sums are fp32); db sums it unrounded.  The order of the
  *        sums is fixed by the sizes and by which of the three are asked for.
  * bias, db: `bias_dtype`, HI3D_F32 or `dtype`.  act: HI3D_ACT_*; GELU is the exact one, QUICK_GELU z * sigmoid(1.702 z).
+ * An operand of one row (M = 1; for w, N = 1) is read at its width, whatever its pitch says.
  * ws: ..._workspace_bytes(d) bytes, 256-byte aligned (that function reads all fields but ws).  Outputs are at any element alignment and overlap nothing.  M = 0: db and dw are zeros, nothing else is written. */
 #define HI3D_ACT_NONE 0
 #define HI3D_ACT_GELU 1

@@ -106,3 +106,14 @@ def test_cpu_tensors_are_refused():
     opt.param_groups[0]["params"][0].grad = x.clone()
     with pytest.raises((RuntimeError, NotImplementedError)):
         opt.step()
+
+
+def test_linear_of_one_row_takes_no_notice_of_its_pitch(lib):
+    """An operand of one row is read where it lies, whatever pitch stands beside it: the same workspace as at its width."""
+    size = lambda **k: lib.hi3d_linear_bwd_workspace_bytes(C.addressof(linear(db=0, z=P, **k)))
+    for act in (0, 1):
+        assert size(M=1, ldx=3, lddy=0, ldz=1, act=act) == size(M=1, ldx=1 << 40, lddy=8, act=act) == size(M=1, act=act)
+        assert size(M=1, K=63, ldx=0, ldw=63, act=act) == size(M=1, K=63, ldx=63, ldw=63, act=act)
+        assert size(N=1, ldw=3, lddy=1, ldz=1, act=act) == size(N=1, lddy=1, ldz=1, act=act)
+    fwd = lambda **k: lib.hi3d_linear_fwd_workspace_bytes(C.addressof(linear(**k)))
+    assert fwd(N=1, ldw=3, ldr=1) == fwd(N=1, ldr=1) == 0

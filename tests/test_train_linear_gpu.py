@@ -371,3 +371,41 @@ def test_a_training_step_of_a_feed_forward_block(dev):
         stale.sum().backward()
     opt.zero_grad()
     assert all(v.grad is None for v in lo.values())
+
+
+@pytest.mark.parametrize("pitch", [0, 1, 8, 40, 1 << 40])
+@pytest.mark.parametrize("M,N,K,act", [(1, 64, 72, "none"), (1, 136, 64, "gelu"), (1, 63, 65, "none"), (40, 1, 64, "none"), (40, 1, 65, "silu"), (1, 1, 8, "none")])
+def test_a_single_row_has_no_pitch(dev, ns, M, N, K, act, pitch):
+    """The C entries take any pitch for an operand of one row and never use it: the same bits as at its width.  dw's contraction runs over the rows of
+    dy and x, dx's over those of w: a row that was read again would be counted again (an infinity times the zeros beside it as NaN)."""
+    import ctypes as C
+    from hi3d_hip import lib as l
+    lib = l.load()
+
+    class Desc(C.Structure):
+        _fields_ = [(n, C.c_void_p) for n in ("x", "w", "bias", "residual", "y", "z", "dy", "dx", "dw", "db")] + \
+                   [(n, C.c_int64) for n in ("M", "ldx", "ldw", "ldr", "lddy", "ldz")] + [(n, C.c_int32) for n in ("N", "K", "dtype", "bias_dtype", "act")] + \
+                   [("ws", C.c_void_p), ("ws_bytes", C.c_int64)]
+    x, w, r, dy, z = (rnd(s, i, "bf16").to(dev) for i, s in enumerate(((M, K), (N, K), (M, N), (M, N), (M, N))))
+    if N == 1:
+        w[0, 3] = float("inf")
+    b = rnd((N,), 9).to(dev)
+    code = {"none": 0, "gelu": 1, "silu": 3}[act]
+    y, kept = ns.linear_act(x, w, b, r, act, True)
+    want = ns.linear_act_bwd(dy, x, w, z, b, act, True, True)
+    if N == 1:
+        assert torch.isinf(want[0][:, 3]).all() and torch.isfinite(want[0][:, :3]).all()
+    out = [torch.zeros_like(t) for t in (y, kept, *want)]
+    m1 = lambda width: pitch if M == 1 else width
+    d = Desc(x=x.data_ptr(), w=w.data_ptr(), bias=b.data_ptr(), residual=r.data_ptr(), y=out[0].data_ptr(), z=out[1].data_ptr(), M=M, ldx=m1(K), ldr=m1(N),
+             ldw=pitch if N == 1 else K, N=N, K=K, dtype=1, bias_dtype=0, act=code)
+    e = Desc(x=x.data_ptr(), w=w.data_ptr(), dy=dy.data_ptr(), z=z.data_ptr(), dx=out[2].data_ptr(), dw=out[3].data_ptr(), db=out[4].data_ptr(), M=M, ldx=m1(K),
+             ldw=pitch if N == 1 else K, lddy=m1(N), ldz=m1(N), N=N, K=K, dtype=1, bias_dtype=0, act=code)
+    st = torch.cuda.current_stream().cuda_stream
+    for desc, size, entry in ((d, lib.hi3d_linear_fwd_workspace_bytes, lib.hi3d_linear_fwd), (e, lib.hi3d_linear_bwd_workspace_bytes, lib.hi3d_linear_bwd)):
+        ws = torch.empty(max(size(C.addressof(desc)), 1), dtype=torch.uint8, device=dev)
+        desc.ws, desc.ws_bytes = ws.data_ptr(), ws.numel()
+        assert entry(C.addressof(desc), st) == 0
+    torch.cuda.synchronize()
+    assert all(torch.equal(p.view(torch.int16) if p.dtype == torch.bfloat16 else p, q.view(torch.int16) if q.dtype == torch.bfloat16 else q)
+               for p, q in zip(out, (y, kept, *want)))
