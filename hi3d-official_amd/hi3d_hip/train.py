@@ -82,6 +82,11 @@ def linear(x, w, bias=None, residual=None, act="none"):
     return _Linear.apply(x.reshape(-1, x.shape[-1]), w, bias, residual, act).reshape(*lead, w.shape[0])
 
 
+def _capturing():
+    """Whether the current stream is being captured into a graph."""
+    return torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
+
+
 class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's update for all tensors of a group in one launch per 72 of them (torch.ops.hi3d.adamw_).
 
@@ -89,7 +94,7 @@ class AdamW(torch.optim.Optimizer):
     working_dtype (torch.bfloat16 / torch.float16): fp32 parameters keep a copy in that type which every step rewrites -- the
     weights that the forward pass reads, `working_copy(p)`, a leaf with a gradient of its own: step() takes that one where p has none.
     capturable: step count on the device (per group: each of its parameters then needs a gradient at every step), so that step() can be
-    captured into a HIP graph; `lr` may then be a one-element fp32 device tensor.  torch.amp.GradScaler's scale and
+    captured into a HIP graph (one that counts on the host refuses: every replay would be the same step); `lr` may then be a one-element fp32 device tensor.  torch.amp.GradScaler's scale and
     overflow flag are read on the device in this mode (it looks at the parameters' own gradients: not together with working copies').
     """
 
@@ -150,6 +155,8 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None):
+        if _capturing() and not all(g["capturable"] for g in self.param_groups):
+            raise _l.Hi3dError("step() is being captured, but a parameter group was not made with capturable=True")
         loss = None
         if closure is not None:
             with torch.enable_grad():

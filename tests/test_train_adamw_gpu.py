@@ -326,3 +326,21 @@ def test_optimiser_with_working_copies_captured(dev):
         train.AdamW(p, lr=lr)
     with pytest.raises(ValueError):
         train.AdamW(p, betas=(1.0, 0.9))
+
+
+def test_a_step_that_counts_on_the_host_is_not_captured(dev):
+    from hi3d_hip import train
+    p = torch.nn.Parameter(torch.randn(100, device=dev))
+    p.grad = torch.randn_like(p)
+    opt = train.AdamW([p], lr=1e-2)
+    opt.step()
+    before, state = p.detach().clone(), {k: v.clone() if torch.is_tensor(v) else v for k, v in opt.state[p].items()}
+    other = torch.zeros(1, device=dev)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        other += 1
+        with pytest.raises(RuntimeError, match="capturable"):
+            opt.step()
+    torch.cuda.synchronize()
+    assert torch.equal(p, before) and all(torch.equal(v, opt.state[p][k]) if torch.is_tensor(v) else v == opt.state[p][k] for k, v in state.items())
+    opt.step()                                   # and goes on outside of it
+    assert opt.state[p]["step"] == 2 and not torch.equal(p, before)

@@ -117,3 +117,48 @@ def test_linear_of_one_row_takes_no_notice_of_its_pitch(lib):
         assert size(N=1, ldw=3, lddy=1, ldz=1, act=act) == size(N=1, lddy=1, ldz=1, act=act)
     fwd = lambda **k: lib.hi3d_linear_fwd_workspace_bytes(C.addressof(linear(**k)))
     assert fwd(N=1, ldw=3, ldr=1) == fwd(N=1, ldr=1) == 0
+
+
+def leaf(n=4, dtype=torch.float32, grad=True):
+    p = torch.nn.Parameter(torch.ones(n, dtype=dtype))
+    if grad:
+        p.grad = torch.ones(n, dtype=dtype)
+    return p
+
+
+class Launches:
+    """In the operators' place: takes what AdamW.step() hands over, refuses where it is told to."""
+    def __init__(self, refuse=()):
+        self.calls, self.refuse = [], list(refuse)
+
+    def adamw_(self, *a):
+        if self.refuse and self.refuse.pop(0):
+            raise RuntimeError("refused")
+        self.calls.append(a)
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    from hi3d_hip import train
+    def put(**k):
+        l = Launches(**k)
+        monkeypatch.setattr(train.torch_ops, "load", lambda: l)
+        return l
+    return put
+
+
+@pytest.fixture
+def capturing(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+
+
+def test_a_step_that_counts_on_the_host_is_not_captured(launches, capturing):
+    """A replay would take the same step number and rate for ever."""
+    from hi3d_hip import train
+    ops = launches()
+    p, q = leaf(), leaf()
+    for opt in (train.AdamW([p, q]), train.AdamW([dict(params=[p], capturable=True), dict(params=[q])])):
+        with pytest.raises(RuntimeError, match="capturable"):
+            opt.step()
+        assert not ops.calls and not opt.state
