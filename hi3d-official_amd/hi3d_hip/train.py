@@ -94,7 +94,8 @@ class AdamW(torch.optim.Optimizer):
     working_dtype (torch.bfloat16 / torch.float16): fp32 parameters keep a copy in that type which every step rewrites -- the
     weights that the forward pass reads, `working_copy(p)`, a leaf with a gradient of its own: step() takes that one where p has none.
     capturable: step count on the device (per group: each of its parameters then needs a gradient at every step), so that step() can be
-    captured into a HIP graph (one that counts on the host refuses: every replay would be the same step); `lr` may then be a one-element fp32 device tensor.  torch.amp.GradScaler's scale and
+    captured into a HIP graph (one that counts on the host refuses: every replay would be the same step) once the state is there -- after an eager step, or
+    after working_copy() of every parameter; `lr` may then be a one-element fp32 device tensor.  torch.amp.GradScaler's scale and
     overflow flag are read on the device in this mode (it looks at the parameters' own gradients: not together with working copies').
     """
 
@@ -128,6 +129,12 @@ class AdamW(torch.optim.Optimizer):
 
     def _state_of(self, p, group):
         s = self.state[p]
+        if "exp_avg" not in s or (group["capturable"] and group["step_t"] is None):
+            # (made in a capture they would be graph nodes: zeroed again by every replay)
+            if _capturing():
+                raise _l.Hi3dError("the optimiser's state cannot be made while a graph is captured: take a step, or every parameter's working_copy(), before")
+            if group["capturable"] and group["step_t"] is None:
+                group["step_t"] = torch.zeros(1, device=p.device)
         if "exp_avg" not in s:
             s["step"] = 0
             s["exp_avg"] = torch.zeros_like(p, dtype=torch.float32)
@@ -163,6 +170,11 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         ns = torch_ops.load()
         scale, found_inf = getattr(self, "grad_scale", None), getattr(self, "found_inf", None)
+        if _capturing():                                     # (all of them, before any is launched)
+            for group in self.param_groups:
+                for p in group["params"]:
+                    if self._grad(p) is not None:
+                        self._state_of(p, group)
         for group in self.param_groups:
             with_grad = [p for p in group["params"] if self._grad(p) is not None]
             if group["capturable"] and with_grad and len(with_grad) < len(group["params"]):
@@ -185,8 +197,6 @@ class AdamW(torch.optim.Optimizer):
             for (dev, step), lists in by_step.items():
                 lr_t = step_t = None
                 if group["capturable"]:
-                    if group["step_t"] is None:
-                        group["step_t"] = torch.zeros(1, device=dev)
                     step_t, lr_t = group["step_t"], group["lr"] if torch.is_tensor(group["lr"]) else None
                 ns.adamw_(*lists, 0.0 if lr_t is not None else float(group["lr"]), b1, b2, group["eps"], group["weight_decay"], max(step, 1), step_t, lr_t,
                           scale if step_t is not None else None, found_inf if step_t is not None else None)

@@ -344,3 +344,38 @@ def test_a_step_that_counts_on_the_host_is_not_captured(dev):
     assert torch.equal(p, before) and all(torch.equal(v, opt.state[p][k]) if torch.is_tensor(v) else v == opt.state[p][k] for k, v in state.items())
     opt.step()                                   # and goes on outside of it
     assert opt.state[p]["step"] == 2 and not torch.equal(p, before)
+
+
+def test_the_first_step_captured(dev):
+    """With the working copies taken beforehand everything that a step keeps is there: replays of a captured first step are the eager steps, and the
+    count goes on from replay to replay.  Without them the capture is refused."""
+    from hi3d_hip import train
+    start = [torch.randn(n, device=dev) for n in (10, 4100)]
+    grads = [[torch.randn_like(t) for t in start] for _ in range(4)]
+    p, q = ([torch.nn.Parameter(t.clone()) for t in start] for _ in range(2))
+    make = lambda params: train.AdamW(params, lr=torch.full((1,), 1e-2, device=dev), working_dtype=torch.bfloat16, capturable=True)
+    opt, eager = make(p), make(q)
+    for a, g in zip(p, grads[0]):
+        a.grad = g.clone()
+    other = torch.zeros(1, device=dev)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        other += 1
+        with pytest.raises(RuntimeError, match="captur"):
+            opt.step()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, t) for a, t in zip(p, start))
+    copies = [opt.working_copy(a) for a in p]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        opt.step()
+    for k in range(4):
+        for a, b, t in zip(p, q, grads[k]):
+            a.grad.copy_(t)
+            b.grad = t.clone()
+        g.replay()
+        eager.step()
+        torch.cuda.synchronize()
+        assert opt.param_groups[0]["step_t"].item() == k + 1
+        for a, b, c in zip(p, q, copies):
+            assert torch.equal(a, b) and torch.equal(c, b.detach().bfloat16())
+            assert all(torch.equal(opt.state[a][n], eager.state[b][n]) for n in ("exp_avg", "exp_avg_sq"))

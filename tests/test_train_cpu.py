@@ -162,3 +162,40 @@ def test_a_step_that_counts_on_the_host_is_not_captured(launches, capturing):
         with pytest.raises(RuntimeError, match="capturable"):
             opt.step()
         assert not ops.calls and not opt.state
+
+
+def test_state_is_not_made_in_a_capture(launches, monkeypatch):
+    """What is made in a capture is made again, as zeros, by every replay: the moments, the working copies and the step count have to be there."""
+    from hi3d_hip import train
+    ops = launches()
+    p, q = leaf(), leaf()
+    opt = train.AdamW([p, q], working_dtype=torch.bfloat16, capturable=True)
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_initialized", lambda: True)
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        for f in (opt.step, lambda: opt.working_copy(p)):
+            with pytest.raises(RuntimeError, match="captur"):
+                f()
+            assert not ops.calls and not any(opt.state.values()) and opt.param_groups[0]["step_t"] is None
+    opt.working_copy(p)                              # q has no state yet
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_initialized", lambda: True)
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(RuntimeError, match="captur"):
+            opt.step()
+        assert not ops.calls and not opt.state.get(q)
+    opt.working_copy(q)
+    count = opt.param_groups[0]["step_t"]
+    assert count is not None and count.item() == 0
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_initialized", lambda: True)
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        opt.step()
+    assert len(ops.calls) == 1 and ops.calls[0][11] is count
+
+
+def test_a_group_without_gradients_needs_no_state_in_a_capture(launches, capturing):
+    from hi3d_hip import train
+    ops = launches()
+    train.AdamW([leaf(grad=False)], capturable=True).step()
+    assert not ops.calls
