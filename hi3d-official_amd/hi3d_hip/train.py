@@ -113,7 +113,11 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"working_dtype must be torch.bfloat16 or torch.float16, not {working_dtype}")
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, working_dtype=working_dtype,
                                       capturable=capturable, step_t=None))
-        self._step_supports_amp_scaling = all(g["capturable"] for g in self.param_groups)
+
+    @property
+    def _step_supports_amp_scaling(self):
+        """GradScaler asks: whether step() divides by its scale, and heeds its overflow flag, by itself (else it does so before the step)."""
+        return all(g["capturable"] for g in self.param_groups)
 
     def working_copy(self, p):
         """The 16-bit copy of parameter p that step() keeps (before the first step: p rounded)."""
@@ -243,4 +247,3 @@ class AdamW(torch.optim.Optimizer):
                     s["copy"] = before["copy"] if "copy" in before else p.detach().to(working_dtype).requires_grad_(p.requires_grad)
                     with torch.no_grad():
                         s["copy"].copy_(saved["copy"] if "copy" in saved and saved["copy"].dtype == working_dtype else p)
-        self._step_supports_amp_scaling = all(g["capturable"] for g in self.param_groups)

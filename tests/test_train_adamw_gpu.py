@@ -379,3 +379,33 @@ def test_the_first_step_captured(dev):
         for a, b, c in zip(p, q, copies):
             assert torch.equal(a, b) and torch.equal(c, b.detach().bfloat16())
             assert all(torch.equal(opt.state[a][n], eager.state[b][n]) for n in ("exp_avg", "exp_avg_sq"))
+
+
+@pytest.mark.parametrize("modes", [(True, True), (True, False), (False, True), (False, False)])
+def test_with_a_loss_scale(dev, modes):
+    """torch.amp.GradScaler over groups that count on the device and on the host, the second added later: the steps of unscaled gradients, and an
+    overflow is a step that nobody takes.  The scale is a power of two: scaled and unscaled gradients have the same digits."""
+    from hi3d_hip import train
+    start = [torch.randn(n, device=dev) for n in (33, 4100)]
+    def make():
+        p = [torch.nn.Parameter(t.clone()) for t in start]
+        opt = train.AdamW([p[0]], lr=1e-2, capturable=modes[0])
+        opt.add_param_group(dict(params=[p[1]], capturable=modes[1]))
+        return p, opt
+    (p, opt), (q, plain) = make(), make()
+    scaler = torch.amp.GradScaler("cuda", init_scale=1024.0, growth_interval=1000)
+    for k in range(4):
+        scaled = scaler.scale(torch.ones(1, device=dev)).item()
+        grads = [torch.randn_like(t) for t in start]
+        for a, b, g in zip(p, q, grads):
+            a.grad, b.grad = g * scaled, g.clone()
+        before = [a.detach().clone() for a in p]
+        if k == 2:
+            p[1].grad[7] = float("inf")
+        scaler.step(opt)
+        scaler.update()
+        if k == 2:
+            assert all(torch.equal(a, t) for a, t in zip(p, before)) and scaler.get_scale() == 512.0
+            continue
+        plain.step()
+        assert all(torch.equal(a, b) for a, b in zip(p, q)), k

@@ -199,3 +199,19 @@ def test_a_group_without_gradients_needs_no_state_in_a_capture(launches, capturi
     ops = launches()
     train.AdamW([leaf(grad=False)], capturable=True).step()
     assert not ops.calls
+
+
+def test_a_group_that_is_added_later_decides_about_the_loss_scale(launches):
+    """Scaled gradients reach step() only where every group reads the scale on the device; a group that counts on the host would not."""
+    from hi3d_hip import train
+    opt = train.AdamW([leaf()], capturable=True)
+    assert opt._step_supports_amp_scaling
+    opt.add_param_group(dict(params=[leaf()], capturable=False))
+    assert not opt._step_supports_amp_scaling
+    opt = train.AdamW([leaf()])
+    assert not opt._step_supports_amp_scaling
+    opt.param_groups[0]["capturable"] = True
+    opt.add_param_group(dict(params=[leaf()], capturable=True))
+    assert opt._step_supports_amp_scaling
+    import copy
+    assert copy.deepcopy(opt)._step_supports_amp_scaling
