@@ -191,19 +191,21 @@ class AdamW(torch.optim.Optimizer):
                 if g.stride() != p.stride():
                     g = torch.empty_like(p, dtype=g.dtype).copy_(g)
                 s = self._state_of(p, group)
-                if not group["capturable"]:
-                    s["step"] += 1
-                lists = by_step.setdefault((p.device, s["step"]), ([], [], [], [], []))
+                step = 0 if group["capturable"] else s["step"] + 1
+                lists, states = by_step.setdefault((p.device, step), (([], [], [], [], []), []))
                 for to, t in zip(lists, (p, g, s["exp_avg"], s["exp_avg_sq"], s.get("copy"))):
                     if t is not None:
                         to.append(t)
+                states.append(s)
             b1, b2 = group["betas"]
-            for (dev, step), lists in by_step.items():
+            for (_, step), (lists, states) in by_step.items():
                 lr_t = step_t = None
                 if group["capturable"]:
                     step_t, lr_t = group["step_t"], group["lr"] if torch.is_tensor(group["lr"]) else None
                 ns.adamw_(*lists, 0.0 if lr_t is not None else float(group["lr"]), b1, b2, group["eps"], group["weight_decay"], max(step, 1), step_t, lr_t,
                           scale if step_t is not None else None, found_inf if step_t is not None else None)
+                for s in states:                            # (a step that was refused is not counted)
+                    s["step"] = step
         return loss
 
     def load_state_dict(self, state_dict):

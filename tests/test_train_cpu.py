@@ -215,3 +215,24 @@ def test_a_group_that_is_added_later_decides_about_the_loss_scale(launches):
     assert opt._step_supports_amp_scaling
     import copy
     assert copy.deepcopy(opt)._step_supports_amp_scaling
+
+
+def test_a_refused_step_is_not_counted(launches):
+    from hi3d_hip import train
+    p, q, r = leaf(), leaf(), leaf(grad=False)
+    opt = train.AdamW([p, q, r])
+    ops = launches(refuse=[True])
+    with pytest.raises(RuntimeError, match="refused"):
+        opt.step()
+    assert [opt.state[t]["step"] for t in (p, q)] == [0, 0]
+    opt.step()
+    assert [opt.state[t]["step"] for t in (p, q)] == [1, 1] and ops.calls[-1][10] == 1
+    r.grad = torch.ones(4)                            # two launches: steps 2 and 1, the second refused
+    ops.refuse = [False, True]
+    with pytest.raises(RuntimeError, match="refused"):
+        opt.step()
+    assert [opt.state[t]["step"] for t in (p, q, r)] == [2, 2, 0]
+    q.grad = q.grad.to_sparse()                       # found among the gradients, before anything is launched
+    with pytest.raises(RuntimeError, match="sparse"):
+        opt.step()
+    assert [opt.state[t]["step"] for t in (p, q, r)] == [2, 2, 0]
