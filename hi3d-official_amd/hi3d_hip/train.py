@@ -140,12 +140,12 @@ class AdamW(torch.optim.Optimizer):
             if group["capturable"] and group["step_t"] is None:
                 group["step_t"] = torch.zeros(1, device=p.device)
         if "exp_avg" not in s:
+            if group["working_dtype"] is not None and p.dtype != torch.float32:
+                raise _l.Hi3dError("a working copy is kept of fp32 parameters only")
             s["step"] = 0
             s["exp_avg"] = torch.zeros_like(p, dtype=torch.float32)
             s["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32)
             if group["working_dtype"] is not None:
-                if p.dtype != torch.float32:
-                    raise _l.Hi3dError("a working copy is kept of fp32 parameters only")
                 s["copy"] = p.detach().to(group["working_dtype"]).requires_grad_(p.requires_grad)
         return s
 

@@ -236,3 +236,16 @@ def test_a_refused_step_is_not_counted(launches):
     with pytest.raises(RuntimeError, match="sparse"):
         opt.step()
     assert [opt.state[t]["step"] for t in (p, q, r)] == [2, 2, 0]
+
+
+def test_a_copy_that_cannot_be_kept_is_refused_every_time(launches):
+    """A working copy is of an fp32 parameter: the second step is refused like the first, and no half of the state is left."""
+    from hi3d_hip import train
+    ops = launches()
+    p, q = leaf(dtype=torch.bfloat16), leaf()
+    opt = train.AdamW([p, q], working_dtype=torch.bfloat16)
+    for f in (opt.step, opt.step, lambda: opt.working_copy(p), lambda: opt.working_copy(p)):
+        with pytest.raises(RuntimeError, match="fp32"):
+            f()
+    assert not ops.calls and not opt.state.get(p)
+    assert opt.working_copy(q).dtype == torch.bfloat16
