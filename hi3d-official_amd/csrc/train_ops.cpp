@@ -104,7 +104,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> add_layernorm_fwd(const Tensor& x, co
 }
 
 std::tuple<Tensor, Tensor, Tensor> layernorm_bwd(const Tensor& dy, const Tensor& z, const Tensor& mean, const Tensor& rstd, const OptTensor& weight,
-                                                 const OptTensor& bias, const OptTensor& dz) {
+                                                 const OptTensor& bias, const OptTensor& dz, bool need_dw, bool need_db) {
   const char* name = "hi3d::layernorm_bwd";
   const NormArgs a = norm_args(z, weight, bias, name);
   want_gpu(dy, z, name);
@@ -121,8 +121,8 @@ std::tuple<Tensor, Tensor, Tensor> layernorm_bwd(const Tensor& dy, const Tensor&
   const Rows ry = rows_of(dy), rz = rows_of(z), rd = has(dz) ? rows_of(*dz) : Rows{Tensor(), 0, 0, 0};
   const Tensor w = dense(weight);
   Tensor dx = at::empty(z.sizes(), z.options()), dw, db;
-  if (has(weight)) dw = at::empty({a.C}, weight->options());
-  if (has(bias)) db = at::empty({a.C}, bias->options());
+  if (has(weight) && need_dw) dw = at::empty({a.C}, weight->options());
+  if (has(bias) && need_db) db = at::empty({a.C}, bias->options());
   const int64_t ws_n = (dw.defined() || db.defined()) ? hi3d_layernorm_bwd_workspace_floats(a.R, a.C, a.dtype) : 0;
   Tensor ws;
   if (ws_n) ws = at::empty({ws_n}, z.options().dtype(at::kFloat));
@@ -322,7 +322,8 @@ void adamw_(at::TensorList params, at::TensorList grads, at::TensorList exp_avg,
 TORCH_LIBRARY_FRAGMENT(hi3d, m) {
   m.def("layernorm_fwd(Tensor x, Tensor? weight, Tensor? bias, float eps) -> (Tensor, Tensor, Tensor)");
   m.def("add_layernorm_fwd(Tensor x, Tensor residual, Tensor? weight, Tensor? bias, float eps) -> (Tensor, Tensor, Tensor, Tensor)");
-  m.def("layernorm_bwd(Tensor dy, Tensor z, Tensor mean, Tensor rstd, Tensor? weight, Tensor? bias, Tensor? dz) -> (Tensor, Tensor, Tensor)");
+  m.def("layernorm_bwd(Tensor dy, Tensor z, Tensor mean, Tensor rstd, Tensor? weight, Tensor? bias, Tensor? dz, bool need_dw=True, "
+        "bool need_db=True) -> (Tensor, Tensor, Tensor)");
   m.def("linear_act(Tensor x, Tensor w, Tensor? bias, Tensor? residual, str act, bool save_z) -> (Tensor, Tensor)");
   m.def("linear_act_bwd(Tensor dy, Tensor x, Tensor w, Tensor? z, Tensor? bias, str act, bool need_dx, bool need_dw) -> (Tensor, Tensor, Tensor)");
   m.def("adamw_(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avg, Tensor(c!)[] exp_avg_sq, Tensor(d!)[] copies, float lr, float beta1, "

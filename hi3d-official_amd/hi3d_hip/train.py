@@ -40,7 +40,7 @@ class _LayerNorm(torch.autograd.Function):
         z, mean, rstd, weight, bias = ctx.saved_tensors
         if dy is None:                               # nothing reads y: the gradient passes through the sum alone
             return dz, dz, None, None, None
-        dx, dw, db = torch_ops.load().layernorm_bwd(dy, z, mean, rstd, weight, bias, dz)
+        dx, dw, db = torch_ops.load().layernorm_bwd(dy, z, mean, rstd, weight, bias, dz, *ctx.needs_input_grad[2:4])
         return dx, dx if ctx.needs_input_grad[1] else None, dw, db, None
 
 

@@ -245,3 +245,36 @@ def test_on_another_stream_and_replayed(dev, ns):
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(out, both()))
+
+
+@pytest.mark.parametrize("R,C,dt", [(7, 40, "bf16"), (1030, 320, "fp16"), (300, 5120, "fp32")])
+def test_frozen_weight_and_bias_cost_nothing(dev, ns, monkeypatch, R, C, dt):
+    """Sums that nobody asks for are not taken, and the others keep their bits."""
+    from hi3d_hip import train
+    z, dy, w, b = rnd((R, C), 1, dt).to(dev), rnd((R, C), 2, dt).to(dev), rnd((C,), 3, "fp32", 0.2, 1.0).to(dev), rnd((C,), 4).to(dev)
+    _, mean, rstd = ns.layernorm_fwd(z, w, b, 1e-5)
+    dx, dw, db = ns.layernorm_bwd(dy, z, mean, rstd, w, b, z)
+    for nw, nb in ((True, True), (True, False), (False, True), (False, False)):
+        got = ns.layernorm_bwd(dy, z, mean, rstd, w, b, z, nw, nb)
+        assert torch.equal(got[0], dx)
+        assert torch.equal(got[1], dw) if nw else got[1] is None
+        assert torch.equal(got[2], db) if nb else got[2] is None
+    asked = []
+
+    class Spy:
+        def __getattr__(self, name):
+            f = getattr(ns, name)
+            def call(*a):
+                out = f(*a)
+                if name == "layernorm_bwd":
+                    asked.append([t is not None for t in out])
+                return out
+            return call
+    monkeypatch.setattr(train.torch_ops, "load", lambda: Spy())
+    for nw, nb in ((True, False), (False, True), (False, False)):
+        x, wp, bp = z.clone().requires_grad_(), w.clone().requires_grad_(nw), b.clone().requires_grad_(nb)
+        train.layer_norm(x, wp, bp).backward(dy)
+        plain = ns.layernorm_bwd(dy, z, mean, rstd, w, b, None)
+        assert asked.pop() == [True, nw, nb] and torch.equal(x.grad, plain[0])
+        assert torch.equal(wp.grad, plain[1]) if nw else wp.grad is None
+        assert torch.equal(bp.grad, plain[2]) if nb else bp.grad is None
