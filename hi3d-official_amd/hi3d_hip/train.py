@@ -53,8 +53,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, bias, residual, act):
-        y, z = torch_ops.load().linear_act(x, w, bias, residual, act, act != "none" and any(ctx.needs_input_grad[:3]))
+    def forward(ctx, x, w, bias, residual, act, recorded):
+        y, z = torch_ops.load().linear_act(x, w, bias, residual, act, recorded and act != "none" and any(ctx.needs_input_grad[:3]))
         ctx.act = act
         ctx.save_for_backward(x, w, bias, z)
         return y
@@ -63,11 +63,11 @@ class _Linear(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, w, bias, z = ctx.saved_tensors
-        nx, nw, nb, nr, _ = ctx.needs_input_grad
+        nx, nw, nb, nr = ctx.needs_input_grad[:4]
         dx = dw = db = None
         if nx or nw or nb:
             dx, dw, db = torch_ops.load().linear_act_bwd(dy, x, w, z, bias if nb else None, ctx.act, nx, nw)
-        return dx, dw, db, dy if nr else None, None
+        return dx, dw, db, dy if nr else None, None, None
 
 
 def linear(x, w, bias=None, residual=None, act="none"):
@@ -79,7 +79,8 @@ def linear(x, w, bias=None, residual=None, act="none"):
         if residual.shape != (*lead, w.shape[0]):
             raise _l.Hi3dError(f"linear: residual must be {tuple(lead) + (w.shape[0],)}, got {tuple(residual.shape)}")
         residual = residual.reshape(-1, w.shape[0])
-    return _Linear.apply(x.reshape(-1, x.shape[-1]), w, bias, residual, act).reshape(*lead, w.shape[0])
+    # (inside forward() the grad mode is off whatever the caller's is, and a leaf needs a gradient under no_grad too)
+    return _Linear.apply(x.reshape(-1, x.shape[-1]), w, bias, residual, act, torch.is_grad_enabled()).reshape(*lead, w.shape[0])
 
 
 def _capturing():

@@ -249,3 +249,25 @@ def test_a_copy_that_cannot_be_kept_is_refused_every_time(launches):
             f()
     assert not ops.calls and not opt.state.get(p)
     assert opt.working_copy(q).dtype == torch.bfloat16
+
+
+def test_z_is_kept_only_for_a_backward_pass(monkeypatch):
+    """Without gradients to come -- no_grad, inference, frozen operands, a gradient for the residual alone -- the activation's argument is not written."""
+    from hi3d_hip import train
+    kept = []
+
+    class Ops:
+        def linear_act(self, x, w, bias, residual, act, save):
+            kept.append(save)
+            return x @ w.t(), x @ w.t() if save else None
+    monkeypatch.setattr(train.torch_ops, "load", lambda: Ops())
+    x, w = torch.ones(2, 3), torch.ones(4, 3, requires_grad=True)
+    r = torch.zeros(2, 4, requires_grad=True)
+    train.linear(x, w, act="gelu")
+    train.linear(x, w, act="none")
+    train.linear(x, w.detach(), residual=r, act="gelu")
+    with torch.no_grad():
+        y = train.linear(x, w, residual=r, act="gelu")
+    with torch.inference_mode():
+        train.linear(x, w, act="silu")
+    assert kept == [True, False, False, False, False] and not y.requires_grad
