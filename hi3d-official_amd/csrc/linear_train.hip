@@ -27,8 +27,9 @@ constexpr long MOST_PITCH = 0x200000, MOST_WIDTH = 0x100000;
 
 // ---- activations ------------------------------------------------------------------------------------------------------------------
 // Phi(-a) = exp(-a^2 / 2) P(t), t = 1 / (1 + 0.3 a), a >= 0: P of degree 8 without constant term, fitted to the Mills ratio over
-// [0, 14] with least relative error, 1.5e-7 (4.6e-7 as evaluated in fp32) -- relative also where Phi is tiny, which an erf with an
-// absolute error would not give, and small enough for the fp32 sums of the bias' gradient.
+// [0, 14] with least relative error, 1.5e-7 -- relative also where Phi is tiny, which an erf with an absolute error would not give, and small enough
+// for the fp32 sums of the bias' gradient.  In fp32 the roundings of the exponent's argument come on top, a^2 2^-24, and a few of 2^-24: 7.5e-7 up to a = 3,
+// 1.6e-6 up to 5, 8e-6 at 13, where Phi leaves fp32's normal numbers.
 __device__ __forceinline__ void gauss(float x, float& cdf, float& bell) {
   const float a = fabsf(x);
   const float t = __builtin_amdgcn_rcpf(1.0f + 0.3f * a);
@@ -44,7 +45,8 @@ __device__ __forceinline__ void gauss(float x, float& cdf, float& bell) {
   q = q * t * bell;
   cdf = x < 0.0f ? q : 1.0f - q;
 }
-// x Phi(x) = max(x, 0) - |x| Phi(-|x|), for results of 16 bits: the same with P of degree 6, 4.7e-6 (a 26th of fp16's half step).  The epilogue of a
+// x Phi(x) = max(x, 0) - |x| Phi(-|x|), for results of 16 bits: the same with P of degree 6, fitted to 4.7e-6; in fp32 5.4e-6 up to |x| = 5 (fp16's half
+// step, 2^-12 ... 2^-11 of a value, is at least 45 times that; its normal numbers end there) and 1.0e-5 at 13.  The epilogue of a
 // 256-row tile is bound by these instructions.  |x| is bounded where it multiplies, so that infinity stays (NaN comes through Phi).
 __device__ __forceinline__ float gelu(float x) {
   const float a = fabsf(x);

@@ -409,3 +409,20 @@ def test_a_single_row_has_no_pitch(dev, ns, M, N, K, act, pitch):
     torch.cuda.synchronize()
     assert all(torch.equal(p.view(torch.int16) if p.dtype == torch.bfloat16 else p, q.view(torch.int16) if q.dtype == torch.bfloat16 else q)
                for p, q in zip(out, (y, kept, *want)))
+
+
+def test_gelus_slope_keeps_its_digits_in_32_bits(dev, ns):
+    """The bias' gradient of one row of ones is the slope itself, not rounded to 16 bits: Phi(z) + z phi(z), |z| <= 13 (beyond, Phi(-|z|) leaves fp32's
+    normal numbers).  Phi(-a): 1.5e-7 of the fit, a^2 2^-24 of the exponent's two roundings (a^2 / 2 each), and 24 roundings for the reciprocal, the
+    exponential (a unit in the last place is two) and 16 steps; a phi(a): the exponent's again and 8; the sum of the two: 2."""
+    z = torch.cat([torch.linspace(-13, 13, 8001), torch.linspace(-1e-2, 1e-2, 99), torch.zeros(1)]).bfloat16()[None]
+    n = z.shape[1]
+    one, w = torch.ones(1, n).bfloat16().to(dev), torch.zeros(n, 8).bfloat16().to(dev)
+    got = ns.linear_act_bwd(one, torch.zeros(1, 8).bfloat16().to(dev), w, z.to(dev), torch.zeros(n, device=dev), "gelu", False, False)[2].double().cpu()
+    z = z[0].double()
+    a = z.abs()
+    tail, bell = torch.special.log_ndtr(-a).exp(), torch.exp(-a * a / 2) * (0.5 / torch.pi) ** 0.5
+    want = torch.where(z < 0, tail, 1 - tail) + z * bell
+    slack = (1.5e-7 + (a * a + 24) * U32) * tail + (a * a + 8) * U32 * a * bell + 2 * U32 * want.abs()
+    off = (got - want).abs() / slack
+    assert (off <= 1).all(), f"worst {off.max().item():.2f} of its tolerance at {z[off.argmax()].item()}"
