@@ -11,7 +11,7 @@ trained through the operator binding:
 
 `AdamW` is a torch.optim.Optimizer and so a `target:` of the reference's YAML (`optimizer_config`).  Underneath are
 torch.ops.hi3d.layernorm_fwd / add_layernorm_fwd / layernorm_bwd / linear_act /
-linear_act_bwd / adamw_, which may be called by themselves: a step that is
+linear_act_bwd / adamw_, which may be called by themselves (they record no gradients): a step that is
 captured into a HIP graph calls these, since a captured autograd backward shares its leaves' gradient nodes -- and the
 stream they were made on -- with any eager graph of the same leaves that is still alive.
 """
@@ -71,9 +71,9 @@ class _Linear(torch.autograd.Function):
 
 
 def linear(x, w, bias=None, residual=None, act="none"):
-    """act(x w^T + bias) (+ residual), differentiable.  x [..., K], w [N, K] (nn.Linear's): bf16 or fp16, any sizes and strides; bias [N]:
-    fp32 or x's type; residual [..., N] of x's type and exactly the result's shape; act: "none", "gelu" (exact), "quick_gelu", "silu",
-    "relu".  Products and sums are fp32; the gradients' products take dy act'(z) rounded to x's type, z being kept in it."""
+    """act(x w^T + bias) (+ residual), differentiable.  x [..., K], w [N, K] (nn.Linear's): both bf16 or both fp16 (nothing is cast, not under autocast
+    either: fp32 parameters take part as 16-bit copies, AdamW's `working_dtype`), any strides, widths up to 1048576; bias [N]: fp32 or x's type; residual [..., N] of x's type and exactly the result's shape; act: "none", "gelu" (exact), "quick_gelu", "silu",
+    "relu".  Products and sums are fp32; the gradients' products take dy act'(z) rounded to x's type, z being kept in it (bias' gradient: not rounded)."""
     lead = x.shape[:-1]
     if residual is not None:
         if residual.shape != (*lead, w.shape[0]):

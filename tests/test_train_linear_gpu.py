@@ -426,3 +426,25 @@ def test_gelus_slope_keeps_its_digits_in_32_bits(dev, ns):
     slack = (1.5e-7 + (a * a + 24) * U32) * tail + (a * a + 8) * U32 * a * bell + 2 * U32 * want.abs()
     off = (got - want).abs() / slack
     assert (off <= 1).all(), f"worst {off.max().item():.2f} of its tolerance at {z[off.argmax()].item()}"
+
+
+def test_a_gated_feed_forward_as_the_unets_have_it(dev):
+    """Linear(C -> 8 C), split, a gelu(g), Linear(4 C -> C) and the residual (attention.py:87-113): both linear layers on the operators, the gate in torch.
+    Result and gradients against 64 bits from the same bf16 weights, relative to their norm, 2^-8 for each bf16 rounding on the way."""
+    from hi3d_hip import train
+    T, C = 154, 80
+    init = dict(w=rnd((8 * C, C), 3, "bf16", C ** -0.5), b=rnd((8 * C,), 4, "fp32", 0.2), v=rnd((C, 4 * C), 5, "bf16", (4 * C) ** -0.5), c=rnd((C,), 6, "fp32", 0.2),
+                y=rnd((2, T // 2, C), 7, "bf16"), z=rnd((2, T // 2, C), 8, "bf16"))
+    p = {k: t.to(dev).requires_grad_() for k, t in init.items()}
+    q = {k: t.to(dev).double().requires_grad_() for k, t in init.items()}
+    gy = rnd((2, T // 2, C), 9, "bf16").to(dev)
+    a, g = train.linear(p["y"], p["w"], p["b"]).chunk(2, dim=-1)
+    out = train.linear(a * F.gelu(g), p["v"], p["c"], residual=p["z"])
+    out.backward(gy)
+    a, g = F.linear(q["y"], q["w"], q["b"]).chunk(2, dim=-1)
+    ref = F.linear(a * F.gelu(g), q["v"], q["c"]) + q["z"]
+    ref.backward(gy.double())
+    assert ((out.double() - ref).norm() / ref.norm()).item() < 4 * 2.0 ** -8              # a and g, gelu(g), the product, the result
+    for k in p:
+        # those, and on the way back the product's gradient, the two that the gate sends (through a product each), and the stored one
+        assert ((p[k].grad.double() - q[k].grad).norm() / q[k].grad.norm()).item() < 9 * 2.0 ** -8, k
