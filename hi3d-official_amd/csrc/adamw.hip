@@ -10,8 +10,8 @@
 // Bound by HBM: p, m, v are read and written once, g is read once.  A launch takes up to TENSORS tensors: their pointers travel in the
 // kernel's arguments (no table in memory that a later step or a replay could find overwritten), each tensor is cut into pieces
 // of PIECE elements, one block each, and a block finds its tensor by bisection of the pieces' running count.
-// Measured: 106 M fp32 parameters with bf16 gradients and copies 573 us (5.2 TB/s; a copy of 2 GiB reaches 4.9); 60 tensors of 240 ... 960 elements
-// 6.2 us of 27 us that the call takes (the dispatcher takes 18 us to hand 240 tensors over).
+// Measured: 106 M fp32 parameters with bf16 gradients and copies 572 us (5.2 TB/s; a copy of 2 GiB reaches 4.9); 60 tensors of 240 ... 960 elements
+// 6.5 us of 28 us that the call takes (the dispatcher takes 18 us to hand 240 tensors over).
 #include "train_common.h"
 
 namespace {

@@ -8,10 +8,10 @@
 // contraction (KC: x and w forward, dz for dx) or across it (KS: w for dx, both for dw), and a KS tile reaches the matrix instruction
 // through gfx950's transposing LDS read, so nothing is transposed in memory.
 //
-// Bound by the matrix instructions where the sizes allow: the K loop of the 256 x 320 tile runs at 1450 TFLOP/s with all CUs at work (the library's
-// product of 8192^3: 1407), LDS reads at 77 % of their rate beside it.  Measured, bf16: 16384 x 1280 -> 5120 forward 178 us (1206 TFLOP/s), dx 153
-// (1405), dw 190 (1130, its contraction split in 3); 65536 x 2560 -> 640 182; 8192^3 801 / 807 / 809; 2048 x 1024 -> 1024 10.2 (421); 16 rows
-// 1280 -> 1280 5.4 us, a launch.  What keeps the first from more is a tile's start and end (about 12 us, four rounds), with GELU about 14 us more.
+// Bound by the matrix instructions where the sizes allow: a step more of K runs at 1400 ... 1460 TFLOP/s with all CUs at work (4096 rows -> 5120 in 256 x 320
+// tiles), and each round of tiles has about 10 us of start and end beside that.  Measured back to back, bf16: 16384 x 1280 -> 5120 forward 193 us (1114 TFLOP/s),
+// dx 160 (1344), dw 205 (1050, its contraction split in 3, 16 us of it the join); 65536 x 2560 -> 640 192; 8192^3 832 / 836 / 847 (the library's products
+// 708 / 832 / 947); 2048 x 1024 -> 1024 10.6 (405); 16 rows 1280 -> 1280 5.6 us, a launch.  GELU and a kept z add 14 us to a round.
 #include "train_common.h"
 
 namespace {
@@ -648,8 +648,11 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, Epilogue e
 }
 
 // What the products need first, in one launch:
-//   dz = dy act'(z), rounded to the operands' type for the matrix instruction (its sums stay fp32), in rows padded with zeros to a multiple of 8
-//   elements; and the column sums of the unrounded dz, one row of partial sums per block row (256 columns x 8 row lanes a block; up to SLOPE_FEW rows
+//   dz = dy act'(z), in rows padded with zeros to a multiple of 8 elements, rounded to the operands' type: the matrix instruction takes 16 bits, as every 16-bit
+//   backward pass does.  This is the one rounding besides that of the stored results: dx and dw are off by 0.0023 of their norm in bf16 and 0.00029 in fp16
+//   where unrounded they would be by 0.0017 and 0.00021 (16384 x 1280 -> 5120, 3083 x 650 -> 1290).  dz as a sum of two 16-bit parts would keep the digits
+//   for twice the products (16384 x 1280 -> 5120: about 360 us on top of 467);
+//   the column sums of the unrounded dz, one row of partial sums per block row (256 columns x 8 row lanes a block; up to SLOPE_FEW rows
 //   64 columns x 32 row lanes, and the sums themselves: one launch less);
 //   up to two operands whose rows cannot be read in place, padded likewise.
 struct SlopeParams {
@@ -724,9 +727,9 @@ __global__ __launch_bounds__(256) void prepare_kernel(const SlopeParams s, int a
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------------
-// Tiles, and what one costs in us: a K step with one block on each CU and with `per_cu`, and a tile's start and end.  From sweeps of every tile and
-// split over M 65 ... 65536, N and K 320 ... 5120, all three products: what the estimate picks is within 10 % of the sweep's best nearly
-// everywhere.  64 x 64: small products whose blocks wait for memory and LDS rather than compute (2048 x 1024 x 1024: 14.8 -> 10.4 us).
+// Tiles, and what one costs in us: a K step with one block on each CU and with `per_cu`, and a tile's start and end.  Fitted to sweeps of every tile and
+// split over M 65 ... 65536, N and K 320 ... 5120, all three products: of 147 products the estimate's pick is within 10 % of the best plan in 125, within 20 %
+// in 145, 25 % over it at worst.  64 x 64: small products whose blocks wait for memory and LDS rather than compute (2048 x 1024 x 1024: 14.8 -> 10.4 us).
 struct Config { int bm, bn, per_cu; double one, full, fixed; };
 constexpr Config CONFIGS[] = {{256, 256, 1, 1.45, 1.45, 10.0}, {256, 320, 1, 1.85, 1.85, 9.0}, {128, 128, 2, 0.85, 1.0, 4.0}, {64, 64, 4, 0.4, 0.65, 3.0}};
 constexpr int CUS = 256, MAX_SPLITS = 32;

@@ -14,7 +14,7 @@
 // time and a row sum is log2(LPR) steps for all of them at once; wider rows are held by the block (LPR = 256 or 512).
 //
 // Measured, bf16 rows with fp32 weights: residual sum + norm of 262144 x 320 126 us (5.3 TB/s; a copy of 2 GiB reaches 4.9), norm of 65536 x 640
-// 27.6 us (6.1 TB/s: half of it stays in the last-level cache), gradients of 65536 x 640 with the residual stream's 72 us (4.7 TB/s, 4 us of it the
+// 27.6 us (6.1 TB/s: half of it stays in the last-level cache), gradients of 65536 x 640 with the residual stream's 72 us (4.7 TB/s, 5 us of it the
 // columns' sums), of 7013 x 1285 fp16 22 us (2.4 TB/s: too few rows to hide a row's latency).
 #include "train_common.h"
 

@@ -348,7 +348,7 @@ int hi3d_layernorm_bwd(const void* dy, const void* z, const void* dz, const void
  *        y, z (NULL: not kept): dense [M][N], `dtype`, each one rounding of the fp32 result
  *   bwd: dz = dy act'(z);  dx = dz w;  dw = dz^T x;  db = sum_m dz    dy [M][N] pitch lddy, z [M][N] pitch ldz (not read for
  *        HI3D_ACT_NONE), dx dense [M][K], dw dense [N][K] (`dtype`), db [N] (`bias_dtype`); each of dx, dw, db may be NULL.
- *        dz is rounded to `dtype` for the products (their sums are fp32); db sums it unrounded.  The order of the
+ *        dz is rounded to `dtype` for the products (their sums are fp32) where there is an activation; db sums it unrounded.  The order of the
  *        sums is fixed by the sizes and by which of the three are asked for.
  * bias, db: `bias_dtype`, HI3D_F32 or `dtype`.  act: HI3D_ACT_*; GELU is the exact one, QUICK_GELU z * sigmoid(1.702 z).
  * An operand of one row (M = 1; for w, N = 1) is read at its width, whatever its pitch says.
