@@ -184,6 +184,8 @@ class AdamW(torch.optim.Optimizer):
             with_grad = [p for p in group["params"] if self._grad(p) is not None]
             if group["capturable"] and with_grad and len(with_grad) < len(group["params"]):
                 raise _l.Hi3dError("capturable: every parameter of the group needs a gradient at every step")
+            if group["capturable"] and len({p.device for p in with_grad}) > 1:
+                raise _l.Hi3dError("capturable: the group's step count is on one device, and so must its parameters be")
             by_step = {}                                    # (one list, unless some parameters had no gradient at earlier steps)
             for p in with_grad:
                 g = self._grad(p)

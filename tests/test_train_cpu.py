@@ -271,3 +271,17 @@ def test_z_is_kept_only_for_a_backward_pass(monkeypatch):
     with torch.inference_mode():
         train.linear(x, w, act="silu")
     assert kept == [True, False, False, False, False] and not y.requires_grad
+
+
+def test_a_count_on_one_device_is_not_taken_for_parameters_on_another(launches):
+    """Refused before the first of the devices has taken the step; counts on the host go by device."""
+    from hi3d_hip import train
+    ops = launches()
+    p, q = leaf(), torch.nn.Parameter(torch.ones(4, device="meta"))
+    q.grad = torch.ones(4, device="meta")
+    opt = train.AdamW([p, q], capturable=True)
+    with pytest.raises(RuntimeError, match="device"):
+        opt.step()
+    assert not ops.calls
+    train.AdamW([p, q]).step()
+    assert len(ops.calls) == 2
